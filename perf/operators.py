@@ -223,8 +223,8 @@ def _plain(s):
     op = s["op"]
     if op == "quantize":
         x = s["H"].float()
-        scale = (x.abs().amax(1) / 127.0).clamp_min(2.0 ** -126)
-        # the quotient in 64 bits: next to a half one step decides
+        # both quotients in 64 bits: the scale is a float32 rounded once, and next to a half one step decides
+        scale = (x.abs().amax(1).double() / 127.0).float().clamp_min(2.0 ** -126)
         q = torch.round(x.double() / scale.double()[:, None]).clamp(-127, 127).to(torch.int8)
         return {"q": q, "scale": scale}
     if op == "int8":
