@@ -84,6 +84,45 @@ class DeviceModel:
         self.out_dim = int(arr[len(layers) - 1].out_dim)
 
 
+class ModelBank:
+    """Several models of one architecture on the device, for batches whose graphs belong to different models
+    (``Engine.forward_bank`` / ``solve_bank``; ``Engine.model_bank`` makes one).  ``layers`` = per layer {"weights": float32
+    [models, 2 * out, in] (both supports' weights, an output column's weights contiguous), "bias": None | float32
+    [models, 2 * out] (0 behind the first half), "act", "in", "out", "q" / "scale": the 8-bit form or None}."""
+
+    def __init__(self, layers, num_models: int, precision: str):
+        self.layers, self.num_models, self.precision = layers, num_models, precision
+        self.in_dim, self.out_dim = layers[0]["in"], layers[-1]["out"]
+
+
+def _matrix(x, what, dtypes, cols=None, rows=None):
+    """Check a 2-D tensor whose rows are contiguous; -> its row stride in elements."""
+    if x.dtype not in dtypes:
+        raise TypeError("%s is %s, expected %s" % (what, x.dtype, " / ".join(str(d) for d in dtypes)))
+    shape = x.shape
+    if len(shape) != 2 or (cols is not None and shape[1] != cols) or (rows is not None and shape[0] != rows):
+        raise ValueError("%s has shape %s, expected [%s, %s]" % (what, tuple(shape), "rows" if rows is None else rows,
+                                                                 "columns" if cols is None else cols))
+    ld, inner = x.stride()
+    if shape[1] > 1 and inner != 1:
+        raise ValueError("%s: the entries of a row must be contiguous" % what)
+    if shape[0] <= 1:
+        return max(int(shape[1]), 1)
+    if ld < shape[1]:
+        raise ValueError("%s: rows overlap (row stride %d, %d columns)" % (what, ld, shape[1]))
+    return ld
+
+
+def _array(x, what, dtype, shape):
+    """Check a contiguous tensor of one dtype and shape."""
+    if x.dtype != dtype:
+        raise TypeError("%s is %s, expected %s" % (what, x.dtype, dtype))
+    if tuple(x.shape) != shape:
+        raise ValueError("%s has shape %s, expected %s" % (what, tuple(x.shape), shape))
+    if not x.is_contiguous():
+        raise ValueError("%s must be contiguous" % what)
+
+
 class Engine:
     def __init__(self, device="cuda"):
         import torch
@@ -239,6 +278,156 @@ class Engine:
                    "dgcn_transform_batch")
         return out
 
+    # ------------------------------------------------------------------ K2/K3 for several models / in 8-bit integers
+    def _codes(self):
+        """{torch dtype: DGCN_* code} of the products' floating-point types."""
+        t = self.torch
+        return {t.float32: _lib.F32, t.bfloat16: _lib.BF16, t.float16: _lib.F16}
+
+    def _here(self, *tensors):
+        """Every tensor (None: not given) lives on this engine's device."""
+        index = self.device.index
+        if index is None:
+            index = self.torch.cuda.current_device()
+        for x in tensors:
+            if x is not None and (x.device.type != self.device.type or x.device.index != index):
+                raise ValueError("a tensor is on %s, the engine on %s" % (x.device, self.device))
+
+    def _launch(self, fn, what, *args):
+        """One library call on this engine's device and current stream."""
+        index = self.device.index
+        if index is None or index == self.torch.cuda.current_device():
+            _lib.check(fn(*args, self._stream()), what)
+        else:
+            with self.torch.cuda.device(index):
+                _lib.check(fn(*args, self._stream()), what)
+
+    def _product_args(self, H, W, bias, act, dtype, out, grouped, rows=None):
+        """The checks every product shares -> (rows, cin, ctot, models, ldh, activation code, dtype code, out, ldy)."""
+        codes = self._codes()
+        if dtype not in codes:
+            raise TypeError("dtype is %s, expected %s" % (dtype, " / ".join(str(d) for d in codes)))
+        if act not in ACT_CODES:
+            raise ValueError("unknown activation %r" % (act,))
+        if W.dim() != (3 if grouped else 2):
+            raise ValueError("the weights have shape %s, expected %s" % (tuple(W.shape), "[models, ctot, cin]" if grouped else "[ctot, cin]"))
+        if not W.is_contiguous():
+            raise ValueError("the weights must be contiguous")
+        ctot, cin = W.shape[-2], W.shape[-1]
+        M = W.shape[0] if grouped else 1
+        ldh = cin
+        if H is not None:
+            ldh = _matrix(H, "H", (W.dtype,), cols=cin, rows=rows)
+            rows = H.shape[0]
+        if bias is not None:
+            _array(bias, "bias", self.torch.float32, (M, ctot) if grouped else (ctot,))
+        if out is None:
+            out, ldy = self.torch.empty((rows, ctot), dtype=dtype, device=self.device), max(ctot, 1)
+        else:
+            ldy = _matrix(out, "out", (dtype,), cols=ctot, rows=rows)
+        self._here(H, W, bias, out)
+        return rows, cin, ctot, M, ldh, ACT_CODES[act], codes[dtype], out, ldy
+
+    def _groups(self, group_ptr, model_of_group, num_models, status):
+        """The arguments every grouped product shares -> (number of groups, status word, is the word this call's own)."""
+        t = self.torch
+        if group_ptr.dim() != 1 or group_ptr.numel() < 1:
+            raise ValueError("group_ptr has shape %s, expected [groups + 1]" % (tuple(group_ptr.shape),))
+        G = group_ptr.numel() - 1
+        _array(group_ptr, "group_ptr", t.int32, (G + 1,))
+        if model_of_group is not None:
+            _array(model_of_group, "model_of_group", t.int32, (G,))
+        elif num_models < G:
+            raise ValueError("%d groups but %d models (and no model_of_group)" % (G, num_models))
+        own = status is None
+        if own:
+            status = t.zeros(1, dtype=t.int32, device=self.device)
+        else:
+            _array(status, "status", t.int32, (1,))
+        self._here(group_ptr, model_of_group, status)
+        return G, status, own
+
+    def quantize_rows(self, X, out=None):
+        """Dynamic 8-bit quantisation of the rows of X (float32 / bfloat16 / float16, any row stride):
+        ``q = X / scale`` rounded half to even, ``scale = max|row| / 127`` (``dgcn_quantize_rows_batch``).  The same call
+        quantises weights, a row per output column.  ``out = (q, scale)`` re-uses buffers.  -> (int8 [rows, cols], float32 [rows]);
+        a row with a NaN or an infinity gets scale NaN."""
+        t = self.torch
+        codes = self._codes()
+        ldx = _matrix(X, "X", tuple(codes))
+        rows, cols = X.shape
+        if out is None:
+            q, scale = t.empty((rows, cols), dtype=t.int8, device=self.device), t.empty(rows, dtype=t.float32, device=self.device)
+            ldq = max(cols, 1)
+        else:
+            q, scale = out
+            ldq = _matrix(q, "q", (t.int8,), cols=cols, rows=rows)
+            _array(scale, "scale", t.float32, (rows,))
+        self._here(X, q, scale)
+        self._launch(self.lib.dgcn_quantize_rows_batch, "dgcn_quantize_rows_batch", X.data_ptr(), codes[X.dtype], ldx, rows, cols,
+                     q.data_ptr(), ldq, scale.data_ptr())
+        return q, scale
+
+    def transform_int8(self, Hq, h_scale, Wq, w_scale, bias=None, act="linear", dtype=None, out=None):
+        """``act((Hq . Wq^T) * h_scale * w_scale + bias)`` (``dgcn_transform_int8_batch``): Hq int8 [rows, cin] with a scale per row,
+        Wq int8 [ctot, cin] (an output column's weights contiguous) with a scale per output column; exact int32 sums, float32 behind
+        them, ``dtype`` (float32 / bfloat16 / float16) out."""
+        t = self.torch
+        if Wq.dtype != t.int8:
+            raise TypeError("Wq is %s, expected torch.int8" % Wq.dtype)
+        rows, cin, ctot, _, ldh, code, dt, out, ldy = self._product_args(
+            Hq, Wq, bias, act, dtype or (t.float32 if out is None else out.dtype), out, False)
+        _array(h_scale, "h_scale", t.float32, (rows,))
+        _array(w_scale, "w_scale", t.float32, (ctot,))
+        self._here(h_scale, w_scale)
+        self._launch(self.lib.dgcn_transform_int8_batch, "dgcn_transform_int8_batch", Hq.data_ptr(), ldh, h_scale.data_ptr(), rows, cin,
+                     Wq.data_ptr(), w_scale.data_ptr(), ctot, None if bias is None else bias.data_ptr(), code, out.data_ptr(), dt, ldy)
+        return out
+
+    def transform_grouped(self, H, W, group_ptr, model_of_group=None, bias=None, act="linear", rows: Optional[int] = None,
+                          h_const: float = 1.0, precise=False, out=None, status=None):
+        """``act(H . W[m]^T + bias[m])``, m the model of the row's group (``dgcn_transform_grouped_batch``): group g owns the rows
+        ``group_ptr[g] .. group_ptr[g + 1]`` (int32 on the device, e.g. a batch's ``graph_ptr``) and takes model
+        ``model_of_group[g]`` (None: model g).  W is [models, ctot, cin] (an output column's weights contiguous), H float32 /
+        bfloat16 / float16 like W, or None for float32 features that all equal ``h_const`` (``rows`` of them).  float32: the bits of
+        ``transform`` with the row's model; ``precise`` as there.  Rows outside every group are left as they were.  With ``status``
+        (an int32 word the caller zeroed) nothing waits and faults are the caller's to read; without, they raise here."""
+        t = self.torch
+        if H is None and (W.dtype != t.float32 or rows is None or rows < 0):
+            raise ValueError("constant features need float32 weights and the number of rows")
+        if precise and W.dtype != t.float32:
+            raise ValueError("precise takes float32")
+        rows, cin, ctot, M, ldh, code, dt, out, ldy = self._product_args(H, W, bias, act, W.dtype, out, True, rows)
+        G, status, own = self._groups(group_ptr, model_of_group, M, status)
+        self._launch(self.lib.dgcn_transform_grouped_batch, "dgcn_transform_grouped_batch", None if H is None else H.data_ptr(), dt, ldh,
+                     float(h_const), rows, cin, group_ptr.data_ptr(), None if model_of_group is None else model_of_group.data_ptr(), G,
+                     W.data_ptr(), M, ctot, None if bias is None else bias.data_ptr(), code, 1 if precise else 0, out.data_ptr(), ldy,
+                     status.data_ptr())
+        if own:
+            self.check_status(status)
+        return out
+
+    def transform_grouped_int8(self, Hq, h_scale, Wq, w_scale, group_ptr, model_of_group=None, bias=None, act="linear", dtype=None,
+                               out=None, status=None):
+        """``transform_int8`` with Wq [models, ctot, cin], w_scale and bias [models, ctot] of the row's model; groups and ``status`` as in
+        ``transform_grouped`` (``dgcn_transform_grouped_int8_batch``)."""
+        t = self.torch
+        if Wq.dtype != t.int8:
+            raise TypeError("Wq is %s, expected torch.int8" % Wq.dtype)
+        rows, cin, ctot, M, ldh, code, dt, out, ldy = self._product_args(
+            Hq, Wq, bias, act, dtype or (t.float32 if out is None else out.dtype), out, True)
+        _array(h_scale, "h_scale", t.float32, (rows,))
+        _array(w_scale, "w_scale", t.float32, (M, ctot))
+        self._here(h_scale, w_scale)
+        G, status, own = self._groups(group_ptr, model_of_group, M, status)
+        self._launch(self.lib.dgcn_transform_grouped_int8_batch, "dgcn_transform_grouped_int8_batch", Hq.data_ptr(), ldh,
+                     h_scale.data_ptr(), rows, cin, group_ptr.data_ptr(), None if model_of_group is None else model_of_group.data_ptr(), G,
+                     Wq.data_ptr(), w_scale.data_ptr(), M, ctot, None if bias is None else bias.data_ptr(), code, out.data_ptr(), dt, ldy,
+                     status.data_ptr())
+        if own:
+            self.check_status(status)
+        return out
+
     # ------------------------------------------------------------------ A4-A6
     def forward(self, b: DeviceBatch, model: DeviceModel, X=None, x_const: Optional[float] = None,
                 mode: int = MODE_LAYERED, out=None):
@@ -270,6 +459,75 @@ class Engine:
                                                    ws.data_ptr(), int(ws.numel()), mode, self._stream()),
                    "dgcn_gcn_forward_batch")
         return out
+
+    def model_bank(self, models, precision: str = "float32") -> ModelBank:
+        """Checkpoints of one architecture ([I, L] supports) as a bank.  ``models``: a list of what ``DeviceModel`` takes (or of
+        objects with such ``.layers``, e.g. ``gcn.models.GCN_DQN``).  ``precision="int8"``: the products of the hidden layers run in 8-bit integers
+        with scales per vertex and output column; the first and the last layer stay in float32 (as do all aggregations)."""
+        t = self.torch
+        models = [getattr(m, "layers", m) for m in models]
+        if not models or not models[0]:
+            raise ValueError("a bank needs at least one model with at least one layer")
+        if precision not in ("float32", "int8"):
+            raise ValueError("precision %r: float32 or int8" % (precision,))
+        shape = lambda m: [([np.shape(w) for w in lyr["weights"]], lyr.get("bias") is not None, ACT_CODES[lyr.get("act")]) for lyr in m]
+        for k, m in enumerate(models):
+            if shape(m) != shape(models[0]):
+                raise ValueError("model %d differs from model 0 in layers, supports, widths, bias or activation" % k)
+        layers = []
+        for l, proto in enumerate(models[0]):
+            if len(proto["weights"]) != 2:
+                raise _lib.DgcnError("a bank takes [I, L] models (max_degree=1); layer %d has %d supports" % (l, len(proto["weights"])))
+            fin, fout = np.shape(proto["weights"][0])
+            if l and fin != layers[-1]["out"]:
+                raise ValueError("layer %d takes %d features, layer %d gives %d" % (l, fin, l - 1, layers[-1]["out"]))
+            W = np.stack([np.concatenate([np.asarray(w, dtype=np.float32) for w in m[l]["weights"]], axis=1).T for m in models])
+            W = t.from_numpy(np.ascontiguousarray(W)).to(self.device)
+            bias = None
+            if proto.get("bias") is not None:
+                bias = np.stack([np.concatenate([np.asarray(m[l]["bias"], dtype=np.float32).ravel(), np.zeros(fout, np.float32)]) for m in models])
+                bias = t.from_numpy(bias).to(self.device)
+            q = scale = None
+            if precision == "int8" and 0 < l < len(models[0]) - 1:
+                q, scale = self.quantize_rows(W.reshape(-1, fin))
+                q, scale = q.reshape(W.shape), scale.reshape(W.shape[:2])
+            layers.append({"weights": W, "bias": bias, "act": proto.get("act"), "in": int(fin), "out": int(fout), "q": q, "scale": scale})
+        return ModelBank(layers, len(models), precision)
+
+    def forward_bank(self, b: DeviceBatch, bank: ModelBank, model_of_graph, X=None, x_const: Optional[float] = None, status=None):
+        """scores[num_nodes, out_dim] of a batch whose graph g belongs to model ``model_of_graph[g]`` (int32 on the device), layer by
+        layer, one product and one aggregation launch each for the whole batch.  A float32 bank without biases returns the bits of
+        ``forward`` with each graph's own model (biases are added before the neighbours' sum here and behind it there); an 8-bit bank is
+        an approximation whose error is the quantisation's.  ``status``: as in ``transform_grouped``."""
+        t = self.torch
+        B, n = b.host.num_graphs, b.host.num_nodes
+        _array(model_of_graph, "model_of_graph", t.int32, (B,))
+        if X is not None:
+            _matrix(X, "X", (t.float32,), cols=bank.in_dim, rows=n)
+        self._here(model_of_graph, X)
+        own = status is None
+        if own:
+            status = t.zeros(1, dtype=t.int32, device=self.device)
+        if n == 0:
+            return t.empty((0, bank.out_dim), dtype=t.float32, device=self.device)
+        if x_const is None:
+            x_const = float(np.float32(1.0 / bank.in_dim))
+        lap = self.supports(b, status=status)
+        H = X
+        for l, lyr in enumerate(bank.layers):
+            out = lyr["out"]
+            if lyr["q"] is not None:
+                q, s = self.quantize_rows(H)
+                Z = self.transform_grouped_int8(q, s, lyr["q"], lyr["scale"], b.graph_ptr, model_of_group=model_of_graph, bias=lyr["bias"],
+                                                status=status)
+            else:
+                Z = self.transform_grouped(H, lyr["weights"], b.graph_ptr, model_of_group=model_of_graph, bias=lyr["bias"], rows=n,
+                                           h_const=x_const, precise=l == 1, status=status)
+            H = self.spmm(lap, Z[:, out:], out, ldz=2 * out, graph_ptr=b.graph_ptr, num_graphs=B, max_nodes=b.host.max_nodes, Y0=Z,
+                          ldy0=2 * out, act=lyr["act"], precise=l == 0)
+        if own:
+            self.check_status(status)
+        return H
 
     def head_dual(self, b: DeviceBatch, act):
         """GCN2_DQN(is_dual=True) output head (gcn/models.py:651-653): [num_nodes, D] -> [num_nodes, D - 1]."""
@@ -347,6 +605,15 @@ class Engine:
         return {"state": state[:, :n], "rounds": rounds[:, :B], "totals": totals[:, :B], "status": status}
 
     # ------------------------------------------------------------------ A10 (batched)
+    def _empty_solution(self, b: DeviceBatch, status):
+        """Nothing but empty graphs: rounds 0, totals 0 (heuristics.py loops do not run)."""
+        t = self.torch
+        B = b.host.num_graphs
+        return {"state": t.empty(0, dtype=t.uint8, device=self.device),
+                "rounds": t.zeros(B, dtype=t.int32, device=self.device),
+                "totals": t.zeros(B, dtype=t.float64, device=self.device), "status": status,
+                "scores": t.empty((0, 1), dtype=t.float32, device=self.device), "stats": None, "overhead": None}
+
     def solve(self, b: DeviceBatch, model: DeviceModel, predict: str = "mwis", mode: int = MODE_LAYERED, X=None,
               x_const=None):
         """GCN forward -> priority -> local greedy for every graph of the batch
@@ -356,19 +623,29 @@ class Engine:
         if model.out_dim != 1:
             raise _lib.DgcnError("solve() needs a model with one output per node (diver_num=1)")
         status = self.torch.zeros(1, dtype=self.torch.int32, device=self.device)
-        if b.host.num_nodes == 0:  # nothing but empty graphs: rounds 0, totals 0 (heuristics.py loops do not run)
-            t = self.torch
-            B = b.host.num_graphs
-            return {"state": t.empty(0, dtype=t.uint8, device=self.device),
-                    "rounds": t.zeros(B, dtype=t.int32, device=self.device),
-                    "totals": t.zeros(B, dtype=t.float64, device=self.device), "status": status,
-                    "scores": t.empty((0, 1), dtype=t.float32, device=self.device), "stats": None, "overhead": None}
+        if b.host.num_nodes == 0:
+            return self._empty_solution(b, status)
         if mode == MODE_FUSED:
             return self.solve_fused(b, model, predict=predict, X=X, x_const=x_const)
         self.supports(b, status=status)  # no host sync on the path: faults surface through res["status"]
         scores = self.forward(b, model, X=X, x_const=x_const, mode=mode)
         res = self.lgs(b, scores=scores, weights=b.weights if predict == "mwis" else None, sum_weights=b.weights,
                        status=status)
+        res["scores"] = scores
+        return res
+
+    def solve_bank(self, b: DeviceBatch, bank: ModelBank, model_of_graph, predict: str = "mwis", X=None, x_const=None):
+        """``solve`` for a batch whose graphs belong to different models: ``forward_bank`` -> priority -> local greedy.  Faults surface
+        through ``res["status"]``."""
+        if b.weights is None:
+            raise ValueError("batch has no vertex weights")
+        if bank.out_dim != 1:
+            raise _lib.DgcnError("solve_bank() needs models with one output per node (diver_num=1)")
+        status = self.torch.zeros(1, dtype=self.torch.int32, device=self.device)
+        scores = self.forward_bank(b, bank, model_of_graph, X=X, x_const=x_const, status=status)
+        if b.host.num_nodes == 0:
+            return self._empty_solution(b, status)
+        res = self.lgs(b, scores=scores, weights=b.weights if predict == "mwis" else None, sum_weights=b.weights, status=status)
         res["scores"] = scores
         return res
 

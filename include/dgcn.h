@@ -37,12 +37,16 @@ enum { DGCN_OK = 0, DGCN_ERR_ARG = -1, DGCN_ERR_LAUNCH = -2, DGCN_ERR_UNSUPPORTE
 /* activation codes (gcn/layers.py:216; tf.nn.leaky_relu alpha = 0.2, gcn/models.py:553) */
 enum { DGCN_ACT_LINEAR = 0, DGCN_ACT_LEAKY_RELU = 1, DGCN_ACT_RELU = 2 };
 
+/* element types of the entry points that take more than float32 */
+enum { DGCN_F32 = 0, DGCN_BF16 = 1, DGCN_F16 = 2 };
+
 /* bits OR-ed into *status by kernels */
 enum {
     DGCN_FAULT_SELF_LOOP = 1,    /* adjacency has a diagonal entry (heuristics.py:94 would loop forever) */
     DGCN_FAULT_NAN_PRIORITY = 2, /* NaN priority (heuristics.py:103-111 never selects it: infinite loop) */
     DGCN_FAULT_DEGREE_RANGE = 4, /* vertex degree >= dinv_table length, or a row with (many) more entries than its graph has vertices */
     DGCN_FAULT_BAD_COLUMN = 8,   /* column id outside the owning graph's node range */
+    DGCN_FAULT_BAD_GROUP = 32,   /* grouped products: group_ptr decreasing or outside [0, rows], or a model id outside [0, num_models) */
     DGCN_FAULT_CLUSTER = 16      /* small batches only (one graph on several workgroups): the workgroups of a graph did not
                                     end up on one XCD, or one of them never arrived - results are not valid; rerun after
                                     dgcn_set_option("fused_cluster", 0) */
@@ -219,6 +223,46 @@ int dgcn_transform_batch(const float* H, int32_t ldh, float h_const, int32_t row
  * contract of LAYER INDEX 1 in every forward / solve entry point below. */
 int dgcn_transform_f64acc_batch(const float* H, int32_t ldh, float h_const, int32_t rows, int32_t cin,
                                 const float* W, int32_t ctot, float* Z, int32_t ldz, void* stream);
+
+/* ---- the same dense products for batches of several models, and in 8-bit integers --------------------------------------
+ * The reference restores one checkpoint per process (mwis_dqn_call.py:188-192) and ships 46 of them; here the graphs of one batch may
+ * belong to different models.  Common to the entry points below:
+ *  - Weights are OUTPUT-major: W[ctot][cin] (one row per output column of the product, its cin weights contiguous; the
+ *    transpose of DgcnLayer.weights), num_models such matrices one behind the other for the grouped forms; bias (or NULL) and
+ *    w_scale are [num_models][ctot] float32.
+ *  - ld* are row strides in elements (ldh >= cin, ldy >= ctot), any alignment the element type has; 64-bit offsets.
+ *  - Groups: group_ptr[num_groups + 1] (device, int32, non-decreasing in [0, rows]; a batch's graph_ptr is one): group g owns rows
+ *    [group_ptr[g], group_ptr[g+1]) and takes model model_of_group[g] (device, int32; NULL: model g).  Groups may be empty; rows
+ *    before the first and behind the last group are left as they were.  DGCN_FAULT_BAD_GROUP in *status (required; the caller
+ *    zeroes it once): a pointer that decreases or leaves [0, rows], a model id outside [0, num_models) - that group's rows are
+ *    left as they were (bad pointers: clamped, contents of Y's rows then undefined).
+ *  - act is applied behind the bias.  No atomics but the status word, no workspace: a row's result depends on that row, its model
+ *    and the call's sizes (rows, num_groups, cin, ctot, types) only, and repeated calls return the same bits.
+ *
+ * dgcn_quantize_rows_batch: Q[r][k] = x / scale[r] rounded half to even (exact quotient), |Q| <= 127;
+ *   scale[r] = max(max_k |X[r][k]| / 127, 2^-126) in float32.  A row with a NaN or an infinity gets scale NaN and Q = 0, so that every
+ *   product of that row is NaN.  X: float32 / bf16 / fp16 (dtype).  Q must not overlap X.
+ * dgcn_transform_int8_batch: Y[r][n] = act(((float)acc * h_scale[r]) * w_scale[n] + bias[n]), acc = sum_k H[r][k] W[n][k] exact in
+ *   int32 (cin <= 131071), float32 arithmetic behind it, rounded once to out_dtype.
+ * dgcn_transform_grouped_batch: Y[r][n] = act(sum_k H[r][k] W[e][n][k] + bias[e][n]), e the model of r's group; H, W and Y are of
+ *   one dtype.  float32: an ascending fmaf chain over k from 0 - the bits of dgcn_transform_batch with that model's weights -,
+ *   precise != 0: the chain in double, rounded once - the bits of dgcn_transform_f64acc_batch; H NULL: every entry is h_const.
+ *   bf16 / fp16: exact products summed in float32, one rounding at the end; precise must be 0 and H not NULL.
+ * dgcn_transform_grouped_int8_batch: the 8-bit product with W, w_scale and bias of the row's model. */
+int dgcn_quantize_rows_batch(const void* X, int32_t dtype, int64_t ldx, int32_t rows, int32_t cols, int8_t* Q, int64_t ldq,
+                             float* scale, void* stream);
+int dgcn_transform_int8_batch(const int8_t* H, int64_t ldh, const float* h_scale, int32_t rows, int32_t cin,
+                              const int8_t* W, const float* w_scale, int32_t ctot, const float* bias, int32_t act,
+                              void* Y, int32_t out_dtype, int64_t ldy, void* stream);
+int dgcn_transform_grouped_batch(const void* H, int32_t dtype, int64_t ldh, float h_const, int32_t rows, int32_t cin,
+                                 const int32_t* group_ptr, const int32_t* model_of_group, int32_t num_groups,
+                                 const void* W, int32_t num_models, int32_t ctot, const float* bias, int32_t act, int32_t precise,
+                                 void* Y, int64_t ldy, int32_t* status, void* stream);
+int dgcn_transform_grouped_int8_batch(const int8_t* H, int64_t ldh, const float* h_scale, int32_t rows, int32_t cin,
+                                      const int32_t* group_ptr, const int32_t* model_of_group, int32_t num_groups,
+                                      const int8_t* W, const float* w_scale, int32_t num_models, int32_t ctot,
+                                      const float* bias, int32_t act, void* Y, int32_t out_dtype, int64_t ldy,
+                                      int32_t* status, void* stream);
 
 /* ---- A4-A6: sess.run(model.outputs_softmax) for a batch (mwis_dqn_call.py:140-143) ------------
  * Precision (part of the ABI, mirrored by oracle/dgcn_oracle.c, identical in every mode and entry point): float32
