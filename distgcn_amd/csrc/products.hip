@@ -6,6 +6,8 @@
 // Every type runs the same tile loop in BYTES: 64 bytes of a row of H and of W feed one step of a 16 x 16 output tile, 16 bytes per
 // lane (lane & 15 = the row, lane >> 4 = which 16 of the 64 bytes): one MFMA of int8 (k = 64), bf16 / fp16 (k = 32), four of float32
 // (k = 4 each).  W is the MFMA's A operand and H its B operand, so a lane ends with four output columns n of ONE row r.
+#include <type_traits>
+
 #include "common.h"
 
 namespace dgcn {
@@ -31,7 +33,7 @@ struct ProductArgs {
     int64_t ldh, ldy;    // elements
     float h_const;
     int rows, cin, ctot, num_groups, num_models, act, out_dtype;
-    bool vec_out;        // rows of Y take 16-byte (float32) / 8-byte (half) stores
+    bool dwords;         // rows of H and W start at multiples of 4 bytes
 };
 
 template <int KIND> struct Elem;
@@ -41,27 +43,113 @@ template <> struct Elem<K_F16> { static constexpr int size = 2; using Acc = f32x
 template <> struct Elem<K_F32> { static constexpr int size = 4; using Acc = f32x4; };
 template <> struct Elem<K_F32P> { static constexpr int size = 4; using Acc = f64x4; };
 
-// The group of a tile slot without a prefix sum over the groups: group g's row tiles start at slot floor(p_g / BM) + g, which is
-// increasing in g, and ceil((p_{g+1} - p_g) / BM) never exceeds the distance to the next group's start.  So a launch of
-// floor(rows / BM) + num_groups slots covers every tile (some slots are empty), and a slot finds its group by search: 64-ary, a lane
-// per probe.  Pointers are clamped to [0, rows] before use: a bad table cannot lead out of the matrix.
-struct Tile { int row0, row1, model; };  // rows [row0, row1) of this slot; row0 >= row1: nothing to do
+struct Tile { int row0, row1, model, col; };  // rows [row0, row1), columns from col on; row0 >= row1: nothing to do
 
-__device__ __forceinline__ Tile find_tile(const ProductArgs& a, int64_t slot, int BM) {
-    Tile t{0, 0, 0};
+// Workgroups go to the XCDs round robin; tile numbers are dealt so that an XCD's workgroups take neighbouring tiles (shared rows of
+// H and W meet in its L2).
+__device__ __forceinline__ int64_t xcd_order(int64_t b, int64_t total) {
+    const int64_t q = total >> 3, r = total & 7, x = b & 7;
+    return x * q + min(x, r) + (b >> 3);
+}
+
+// Tile number b of slots x col_tiles -> slot; `col` <- column tile.  Four slots side by side, column by column: a square-ish patch is in
+// flight at a time.
+__device__ __forceinline__ int64_t patch_order(int64_t b, int64_t slots, int col_tiles, int& col) {
+    const int64_t tile = xcd_order(b, slots * col_tiles);
+    if (col_tiles == 1) { col = 0; return tile; }
+    const int64_t first = tile / (4 * (int64_t)col_tiles) * 4;
+    const int h = (int)min((int64_t)4, slots - first), in = (int)(tile - first * col_tiles);
+    col = in / h;
+    return first + in % h;
+}
+
+__device__ __forceinline__ bool bad_group(const ProductArgs& a, int p0, int p1, int e) {
+    return p0 < 0 || p1 < p0 || p1 > a.rows || e < 0 || e >= a.num_models;
+}
+
+// Up to 256 groups: every wave reads the whole table, four groups per lane, and counts their row tiles, so that every workgroup up to
+// the number of tiles has one (at most min(rows, floor(rows / BM) + num_groups) x column tiles) and the XCDs' shares are equal.  Whole
+// tiles come first, the groups' shorter last tiles behind them: those fill the launch's last round.  Workgroup 0 reports bad entries.
+// Pointers are clamped to [0, rows] before use: a bad table cannot lead out of the matrix.
+constexpr int kCountedGroups = 256;
+template <int BM> __device__ __forceinline__ Tile find_tile_counted(const ProductArgs& a, int64_t b, int col_tiles) {
+    constexpr int N = kCountedGroups / 64;
+    const int lane = threadIdx.x & 63;
+    const int per = (a.num_groups + 63) >> 6;
+    int p[N], len[N], e[N], whole = 0, part = 0;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int g = lane * per + i;
+        p[i] = len[i] = 0;
+        e[i] = -1;
+        if (i < per && g < a.num_groups) {
+            const int v0 = a.gptr[g], v1 = a.gptr[g + 1];
+            e[i] = a.mog ? a.mog[g] : g;
+            bad |= bad_group(a, v0, v1, e[i]);
+            p[i] = min(max(v0, 0), a.rows);
+            len[i] = max(min(max(v1, 0), a.rows) - p[i], 0);
+        }
+        whole += len[i] / BM;
+        part += len[i] % BM != 0;
+    }
+    if (b == 0 && bad) atomicOr(a.status, (int)DGCN_FAULT_BAD_GROUP);
+    int whole_upto = whole, part_upto = part;  // this lane's and all before
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int w = __shfl_up(whole_upto, d), q = __shfl_up(part_upto, d);
+        if (lane >= d) { whole_upto += w; part_upto += q; }
+    }
+    const int64_t all_whole = __builtin_amdgcn_readlane(whole_upto, 63), all_part = __builtin_amdgcn_readlane(part_upto, 63);
+    Tile t{0, 0, 0, 0};
+    const bool in_whole = b < all_whole * col_tiles;
+    if (!in_whole) b -= all_whole * col_tiles;
+    if (!in_whole && b >= all_part * col_tiles) return t;
+    const int slot = (int)patch_order(b, in_whole ? all_whole : all_part, col_tiles, t.col);
+    const int upto = in_whole ? whole_upto : part_upto;
+    const int owner = __builtin_ctzll(__ballot(upto > slot));
+    int at = slot - (upto - (in_whole ? whole : part)), q0 = 0, q1 = 0, qe = -1;  // (meant for the owner: which of its tiles)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int n = in_whole ? len[i] / BM : len[i] % BM != 0;
+        if (at >= 0 && at < n) {
+            q0 = p[i] + (in_whole ? at : len[i] / BM) * BM;
+            q1 = min(q0 + BM, p[i] + len[i]);
+            qe = e[i];
+        }
+        at -= n;
+    }
+    q0 = __builtin_amdgcn_readlane(q0, owner); q1 = __builtin_amdgcn_readlane(q1, owner); qe = __builtin_amdgcn_readlane(qe, owner);
+    if (qe < 0 || qe >= a.num_models) return t;
+    t.row0 = q0;
+    t.row1 = q1;
+    t.model = qe;
+    return t;
+}
+
+// More groups: no count at all.  Group g's row tiles start at slot floor(p_g / BM) + g, which is increasing in g, and
+// ceil((p_{g+1} - p_g) / BM) never exceeds the distance to the next group's start.  So floor(rows / BM) + num_groups slots cover every
+// tile (some slots are empty), and a slot finds its group by search: 64-ary, a lane per probe.  Slot g < num_groups checks entry g.
+template <int BM> __device__ __forceinline__ Tile find_tile(const ProductArgs& a, int64_t b, int64_t slots, int col_tiles) {
+    if (a.gptr && a.num_groups <= kCountedGroups) return find_tile_counted<BM>(a, b, col_tiles);
+    Tile t{0, 0, 0, 0};
+    const int64_t slot = patch_order(b, slots, col_tiles, t.col);
     if (!a.gptr) {
-        const int64_t r = slot * BM;
-        t.row0 = (int)min(r, (int64_t)a.rows);
-        t.row1 = (int)min(r + BM, (int64_t)a.rows);
+        t.row0 = (int)(slot * BM);
+        t.row1 = (int)min(slot * BM + BM, (int64_t)a.rows);
         return t;
     }
+    if (t.col == 0 && slot < a.num_groups && threadIdx.x == 0) {
+        const int g = (int)slot;
+        if (bad_group(a, a.gptr[g], a.gptr[g + 1], a.mog ? a.mog[g] : g)) atomicOr(a.status, (int)DGCN_FAULT_BAD_GROUP);
+    }
     const int lane = threadIdx.x & 63;
-    auto ptr = [&](int g) { return min(max(a.gptr[g], 0), a.rows); };
+    auto clamp = [&](int p) { return min(max(p, 0), a.rows); };
     int lo = 0, n = a.num_groups;  // the group is in [lo, lo + n)
-    while (n > 1) {
+    while (n > 64) {
         const int step = (n + 63) >> 6;
         const int64_t i = (int64_t)lane * step;
-        const bool below = i < n && (int64_t)(ptr(lo + (int)i) / BM) + lo + i <= slot;
+        const bool below = i < n && (int64_t)(clamp(a.gptr[lo + (i < n ? (int)i : 0)]) / BM) + lo + i <= slot;
         const unsigned long long m = __ballot(below);
         const int k = m == ~0ull ? 64 : __builtin_ctzll(~m);
         if (k == 0) return t;  // in front of the first group
@@ -69,24 +157,20 @@ __device__ __forceinline__ Tile find_tile(const ProductArgs& a, int64_t slot, in
         lo += at;
         n = min(step, n - at);
     }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    const int p0 = ptr(lo), p1 = ptr(lo + 1);
-    const int64_t tile = slot - (p0 / BM + (int64_t)lo);
-    const int64_t r = p0 + tile * BM;
-    if (tile < 0 || r >= p1) return t;
-    const int e = a.mog ? a.mog[lo] : lo;
-    if (e < 0 || e >= a.num_models) return t;
+    // at most 64 candidates: a lane each, its pointers and model number with it
+    const int g = lo + min(lane, n - 1);
+    const int p0 = clamp(a.gptr[g]), p1 = clamp(a.gptr[g + 1]), e = a.mog ? a.mog[g] : g;
+    const unsigned long long m = __ballot(lane < n && (int64_t)(p0 / BM) + g <= slot);
+    const int k = m == ~0ull ? 64 : __builtin_ctzll(~m);
+    if (k == 0) return t;
+    const int at = __builtin_amdgcn_readfirstlane(k - 1);
+    const int q0 = __builtin_amdgcn_readlane(p0, at), q1 = __builtin_amdgcn_readlane(p1, at), qe = __builtin_amdgcn_readlane(e, at);
+    const int64_t r = q0 + (slot - (q0 / BM + (int64_t)lo + at)) * BM;
+    if (r < q0 || r >= q1 || qe < 0 || qe >= a.num_models) return t;
     t.row0 = (int)r;
-    t.row1 = (int)min(r + BM, (int64_t)p1);
-    t.model = e;
+    t.row1 = (int)min(r + BM, (int64_t)q1);
+    t.model = qe;
     return t;
-}
-
-// Every slot below num_groups checks the table entry of its own number.
-__device__ __forceinline__ void check_group(const ProductArgs& a, int64_t slot) {
-    if (!a.gptr || slot >= a.num_groups || threadIdx.x != 0) return;
-    const int g = (int)slot, p0 = a.gptr[g], p1 = a.gptr[g + 1], e = a.mog ? a.mog[g] : g;
-    if (p0 < 0 || p1 < p0 || p1 > a.rows || e < 0 || e >= a.num_models) atomicOr(a.status, (int)DGCN_FAULT_BAD_GROUP);
 }
 
 template <int KIND>
@@ -106,180 +190,711 @@ __device__ __forceinline__ typename Elem<KIND>::Acc mfma_step(i32x4 w, i32x4 h, 
 }
 
 // A lane's 16 bytes of a 64-byte step.  float32 takes element 4 s + (lane >> 4) for MFMA s (the chain is then ascending in k);
-// the other types take chunk lane >> 4 as it lies.  `row` is the LDS row, `step` the 64-byte step within it.
+// the other types take chunk lane >> 4 as it lies.  `row` is the LDS row, `key` its chunk permutation, `step` the 64-byte step.
 template <int KIND, int ROW_BYTES>
-__device__ __forceinline__ i32x4 lds_frag(const char* base, int row, int step) {
+__device__ __forceinline__ i32x4 lds_frag(const char* base, int row, int key, int step) {
     const int q = (threadIdx.x & 63) >> 4;
     if constexpr (KIND == K_F32 || KIND == K_F32P) {
         i32x4 v;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) v[s] = *reinterpret_cast<const int*>(base + row * ROW_BYTES + (((step * 4 + s) ^ (row & 7)) << 4) + (q << 2));
+        for (int s = 0; s < 4; ++s) v[s] = *reinterpret_cast<const int*>(base + row * ROW_BYTES + (((step * 4 + s) ^ key) << 4) + (q << 2));
         return v;
     } else {
-        return *reinterpret_cast<const i32x4*>(base + row * ROW_BYTES + (((step * 4 + q) ^ (row & 7)) << 4));
+        return *reinterpret_cast<const i32x4*>(base + row * ROW_BYTES + (((step * 4 + q) ^ key) << 4));
     }
 }
 
-template <class O> __device__ __forceinline__ O round_to(float x) { return (O)x; }
-
-// Four output columns n .. n + 3 of row r.
-template <class O>
-__device__ __forceinline__ void store4(const ProductArgs& a, int64_t r, int n, const float (&v)[4]) {
-    O* y = reinterpret_cast<O*>(a.Y) + r * a.ldy + n;
-    if (a.vec_out && n + 4 <= a.ctot) {
-        using V = __attribute__((ext_vector_type(4))) O;
-        V o;
+// CH output columns n .. n + CH - 1 of row r: scales, bias, activation, one rounding.  `ws`, `bias`: those columns' values.
+template <int KIND, class O, int CH>
+__device__ __forceinline__ void finish(const ProductArgs& a, int64_t r, int n, const float (&v)[CH], float hs, const float (&ws)[CH],
+                                       const float (&bias)[CH]) {
+    using V = __attribute__((ext_vector_type(CH))) O;
+    V o;
+    const bool relu = a.act == DGCN_ACT_RELU;
+    const float slope = a.act == DGCN_ACT_LEAKY_RELU ? kLeakyAlpha : 1.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = round_to<O>(v[i]);
-        *reinterpret_cast<V*>(y) = o;
+    for (int i = 0; i < CH; ++i) {
+        float x = v[i];
+        if constexpr (KIND == K_I8) x = (x * hs) * ws[i];
+        x += bias[i];
+        x = x > 0.f ? x : relu ? 0.f : x * slope;
+        o[i] = (O)x;
+    }
+    O* y = reinterpret_cast<O*>(a.Y) + r * a.ldy + n;
+    if (n + CH <= a.ctot) {
+        __builtin_memcpy(y, &o, sizeof(o));
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < a.ctot) y[i] = round_to<O>(v[i]);
+        for (int i = 0; i < CH - 1; ++i)
+            if (n + i < a.ctot) y[i] = o[i];
     }
 }
 
-// Columns n .. n + 3 of row r from their accumulators: scales, bias, activation, one rounding.
-template <int KIND>
-__device__ __forceinline__ void finish4(const ProductArgs& a, const Tile& t, int64_t r, int n, typename Elem<KIND>::Acc acc) {
-    const int64_t ch = (int64_t)t.model * a.ctot + n;
-    float v[4];
+__device__ const float g_minus_zero = -0.f;
+
+// Scales and biases of the columns n .. n + CH - 1 of a model (the last column's again behind the end).  Without a bias -0 is added:
+// it changes no value, +0 would turn -0 into +0.
+template <int KIND, int CH>
+__device__ __forceinline__ void column_values(const ProductArgs& a, int model, int n, float (&ws)[CH], float (&bias)[CH]) {
+    const int64_t base = (int64_t)model * a.ctot;
+    const float* b = a.bias ? a.bias + base : &g_minus_zero;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[i] = (float)acc[i];
-        const bool in = n + i < a.ctot;
-        if constexpr (KIND == K_I8) v[i] = (v[i] * a.hs[r]) * (in ? a.ws[ch + i] : 0.f);
-        if (a.bias) v[i] += in ? a.bias[ch + i] : 0.f;
-        v[i] = apply_act(v[i], a.act);
+    for (int i = 0; i < CH; ++i) {
+        const int c = min(n + i, a.ctot - 1);
+        ws[i] = KIND == K_I8 ? a.ws[base + c] : 0.f;
+        bias[i] = b[a.bias ? c : 0];
     }
-    if (a.out_dtype == DGCN_F32) store4<float>(a, r, n, v);
-    else if (a.out_dtype == DGCN_BF16) store4<__bf16>(a, r, n, v);
-    else store4<_Float16>(a, r, n, v);
 }
 
-// 16 bytes at byte offset `off` of a row of `row_bytes` bytes; bytes behind the row's end are zero.
-template <int KIND>
+// One wave's TM x TN tiles.  Columns come in pairs of tiles where TN is even (see w_row): a lane holds 8 neighbouring columns.
+template <int KIND, class O, int TM, int TN>
+__device__ __forceinline__ void write_tiles(const ProductArgs& a, const Tile& t, int row, int col, const typename Elem<KIND>::Acc (&acc)[TM][TN]) {
+    constexpr int PW = TN % 2 == 0 && KIND != K_F32P ? 2 : 1, CH = 4 * PW;
+    const int lane = threadIdx.x & 63, q = lane >> 4;
+    float hs[TM];
+    if constexpr (KIND == K_I8) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) hs[i] = a.hs[t.row0 + (int64_t)min(row + i * 16 + (lane & 15), t.row1 - 1 - t.row0)];
+    }
+#pragma unroll
+    for (int p = 0; p < TN / PW; ++p) {
+        const int n = col + p * 16 * PW + q * CH;
+        if (n >= a.ctot) continue;
+        float ws[CH], bias[CH];
+        column_values<KIND, CH>(a, t.model, n, ws, bias);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const int64_t r = (int64_t)t.row0 + row + i * 16 + (lane & 15);
+            if (r >= t.row1) continue;
+            float v[CH];
+#pragma unroll
+            for (int x = 0; x < CH; ++x) v[x] = (float)acc[i][p * PW + (x >> 2)][x & 3];
+            finish<KIND, O, CH>(a, r, n, v, KIND == K_I8 ? hs[i] : 0.f, ws, bias);
+        }
+    }
+}
+
+// The output column (within a wave's columns) that MFMA row i of tile j computes.  An MFMA leaves rows 4 q .. 4 q + 3 in lane group q
+// (double: rows q, q + 4, ..): tiles in pairs deal their columns so that a lane group's 8 (alone: 4) are neighbours.
+template <int KIND, int TN> __device__ __forceinline__ int w_row(int i, int j) {
+    if constexpr (KIND == K_F32P) return j * 16 + 4 * (i & 3) + (i >> 2);
+    else if constexpr (TN % 2 == 0) return (j >> 1) * 32 + (i >> 2) * 8 + (j & 1) * 4 + (i & 3);
+    else return j * 16 + i;
+}
+// The chunk permutation of an LDS row of W: eight lanes in a row read eight different bank groups.
+template <int KIND, int TN> __device__ __forceinline__ int w_key(int row) {
+    if constexpr (TN % 2 == 0 && KIND != K_F32P) return (row & 3) | ((row >> 1) & 4);
+    else return row & 7;
+}
+
+// 16 bytes at byte offset `off` of a row of `row_bytes` bytes, any alignment; bytes behind the row's end are zero: a chunk that crosses
+// the end is the row's last 16 bytes, shifted down.
 __device__ __forceinline__ i32x4 load_chunk(const char* row, int64_t off, int64_t row_bytes) {
-    i32x4 v = {0, 0, 0, 0};
-    if (off + 16 <= row_bytes) {
-        __builtin_memcpy(&v, row + off, 16);
-    } else if (off < row_bytes) {
-        char* d = reinterpret_cast<char*>(&v);
-        constexpr int ES = Elem<KIND>::size;
-#pragma unroll
-        for (int i = 0; i < 16 / ES; ++i)
-            if (off + (i + 1) * ES <= row_bytes) __builtin_memcpy(d + i * ES, row + off + i * ES, ES);
+    unsigned long long u0 = 0, u1 = 0;
+    int64_t over = off;  // how far the chunk lies behind what has been loaded
+    if (row_bytes >= 16) {
+        over = max(off - (row_bytes - 16), (int64_t)0);
+        __builtin_memcpy(&u0, row + (off - over), 8);
+        __builtin_memcpy(&u1, row + (off - over) + 8, 8);
+    } else {
+        for (int i = 0; i < (int)row_bytes; ++i) {
+            const unsigned long long byte = (unsigned char)row[i];
+            if (i < 8) u0 |= byte << (i * 8);
+            else u1 |= byte << (i * 8 - 64);
+        }
     }
-    return v;
+    const int sh = (int)min(over, (int64_t)16) * 8;  // 0 .. 128
+    const unsigned long long lo = sh >= 128 ? 0 : sh >= 64 ? u1 >> (sh - 64) : (u0 >> sh) | ((u1 << 1) << (63 - sh));
+    const unsigned long long hi = sh >= 64 ? 0 : u1 >> sh;
+    return i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
 }
 
-// The general kernel: any alignment, any size.  64 x 64 output tile, four waves of 32 x 32, 128 bytes of k per stage through
-// registers into LDS (rows of 128 bytes, their 16-byte chunks permuted by the row number: reads of eight rows meet no bank twice).
-template <int KIND>
-__global__ __launch_bounds__(256) void k_product_any(ProductArgs a, int64_t slots, int col_tiles) {
-    constexpr int BM = 64, BN = 64, RB = 128, ES = Elem<KIND>::size;
+// The same for a chunk that lies at least 16 bytes behind its row's start and ends at least 4 bytes in front of its end, in rows that
+// start at any byte: five aligned dwords, shifted by the address' low bits.  (A 16-byte load from an address that is no multiple of 4
+// takes several times as long.)
+struct Dwords { i32x4 v; int v4; };
+__device__ __forceinline__ Dwords load_dwords(const char* p) {
+    const char* d = reinterpret_cast<const char*>(__builtin_assume_aligned(p - ((uintptr_t)p & 3), 4));
+    Dwords r;
+    __builtin_memcpy(&r.v, d, 16);
+    __builtin_memcpy(&r.v4, d + 16, 4);
+    return r;
+}
+__device__ __forceinline__ i32x4 shift_dwords(const Dwords& r, int by) {
+    return i32x4{(int)__builtin_amdgcn_alignbyte(r.v[1], r.v[0], by), (int)__builtin_amdgcn_alignbyte(r.v[2], r.v[1], by),
+                 (int)__builtin_amdgcn_alignbyte(r.v[3], r.v[2], by), (int)__builtin_amdgcn_alignbyte(r.v4, r.v[3], by)};
+}
+
+__device__ __attribute__((aligned(16))) const int g_zeros[4] = {0, 0, 0, 0};
+
+// Every wave of the workgroup is here, with its LDS accesses (DIRECT: and all but the last LATER of its loads to LDS) done.
+template <bool DIRECT, int LATER> __device__ __forceinline__ void arrive_all() {
+    if constexpr (DIRECT) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
+    else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+constexpr int kCUs = 256;
+constexpr int kRowBytes = 128;  // bytes of k per stage and row
+
+// One output tile of BM rows x BN columns per workgroup, WM x WN waves.  128 bytes of k per stage, two LDS buffers: while the waves
+// multiply out of one, the next stage travels into the other - DIRECT: by load-to-LDS instructions (rows of H and W at 16-byte
+// strides, a tile's rows within 2 GB), otherwise through registers (any alignment, H == NULL).  An LDS row's eight 16-byte chunks are permuted by the row
+// number, so that eight rows read at one k meet eight bank groups.
+// A stage is worked off in phases (64 bytes of k x up to four row tiles).  AHEAD (the largest tile, two waves per SIMD): a phase's
+// fragments are requested behind the first MFMAs of the phase in front of it, across the stage's barrier too, so the matrix pipe
+// does not wait for LDS; smaller tiles have more waves to hide that.  Row tiles behind the group's last row are skipped four at a time.
+template <int KIND, int BM, int BN, int WM, int WN, int NBUF, bool DIRECT>
+__device__ __forceinline__ void product_tile(const ProductArgs& a, int64_t slots, int col_tiles, char* smem) {
+    constexpr int T = WM * WN * 64, RB = kRowBytes, ES = Elem<KIND>::size;
+    constexpr int TM = BM / WM / 16, TN = BN / WN / 16;       // 16 x 16 tiles per wave
+    constexpr int NH = BM * 8 / T, NW = (BN * 8 + T - 1) / T;  // chunks per thread and stage
+    static_assert(NH * T == BM * 8, "H chunks divide evenly");
+    constexpr int RT = TM <= 4 ? TM : TM / 2, HALVES = TM / RT, PHASES = 2 * HALVES;
+    static_assert(HALVES * RT == TM, "row tiles divide into phases");
     using Acc = typename Elem<KIND>::Acc;
-    __shared__ __attribute__((aligned(16))) char sH[BM * RB];
-    __shared__ __attribute__((aligned(16))) char sW[BN * RB];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
+    constexpr int BUF = (BM + BN) * RB;  // smem: two buffers (one if there is one stage) of [BM rows of H | BN rows of W]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
     const int64_t kbytes = (int64_t)a.cin * ES;
     const int steps = (int)((kbytes + RB - 1) / RB);
-    for (int64_t tile = blockIdx.x; tile < slots * col_tiles; tile += gridDim.x) {
-        const int64_t slot = tile / col_tiles;
-        const int n0 = (int)(tile - slot * col_tiles) * BN;
-        if (n0 == 0) check_group(a, slot);
-        const Tile t = find_tile(a, slot, BM);
-        if (t.row0 >= t.row1) continue;
-        const char* Wm = a.W + (int64_t)t.model * a.ctot * kbytes;
-        Acc acc[2][2] = {};
-        const int lr = threadIdx.x >> 3, lc = threadIdx.x & 7;  // this thread's chunk of rows lr and lr + 32
-        i32x4 h[2], w[2];
-        auto load = [&](int st) {
-            const int64_t off = (int64_t)st * RB + lc * 16;
+
+    const Tile t = find_tile<BM>(a, blockIdx.x, slots, col_tiles);
+    if (t.row0 >= t.row1) return;
+    const int n0 = t.col * BN;
+    const char* Wm = a.W + (int64_t)t.model * a.ctot * kbytes;
+
+    // this thread's chunks: number c of the buffer lies at byte 16 c, row c / 8, and holds chunk (c % 8) ^ (row's key) of that row
+    const char* src[DIRECT ? 1 : NH + NW];
+    int at0[DIRECT ? NH + NW : 1];  // DIRECT: byte offset from the tile's first row
+    int koff[NH + NW];
+    const char* Ht = a.H + (int64_t)t.row0 * a.ldh * ES;
+    const char* Wt = Wm + n0 * kbytes;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int r = min(t.row0 + lr + 32 * j, t.row1 - 1), n = min(n0 + lr + 32 * j, a.ctot - 1);
-                w[j] = load_chunk<KIND>(Wm + (int64_t)n * kbytes, off, kbytes);
-                if ((KIND == K_F32 || KIND == K_F32P) && !a.H) {
+    for (int i = 0; i < NH + NW; ++i) {
+        const bool is_h = i < NH;
+        const int c = (is_h ? i : i - NH) * T + tid, row = c >> 3;
+        koff[i] = ((c & 7) ^ (is_h ? row & 7 : w_key<KIND, TN>(row))) << 4;
+        const int64_t off = is_h ? min(row, t.row1 - 1 - t.row0) * (a.ldh * ES) : min(row, a.ctot - 1 - n0) * kbytes;
+        if constexpr (DIRECT) at0[i] = (int)off + koff[i];
+        else src[i] = (is_h ? Ht : Wt) + off;
+    }
+    constexpr bool W_PART = NW * T != BN * 8;  // the last W chunk belongs to the first waves only
+    i32x4 reg[DIRECT ? 1 : NH + NW];
+    __amdgpu_buffer_rsrc_t rH, rW;
+    if constexpr (DIRECT) {
+        rH = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(Ht), 0, 0x7fffffff, 0x00020000);
+        rW = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(Wt), 0, 0x7fffffff, 0x00020000);
+    }
+    auto fetch = [&](int st, int buf) {
+        const bool whole = (int64_t)(st + 1) * RB <= kbytes;
+        const int at = st * RB;
+        if constexpr (DIRECT) {
+            char* base = smem + buf * BUF + wave * 1024;
+            if (whole) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) h[j][i] = off + 4 * i < kbytes ? __builtin_bit_cast(int, a.h_const) : 0;
+                for (int i = 0; i < NH + NW; ++i) {
+                    if (W_PART && i == NH + NW - 1 && (i - NH) * T + wave * 64 >= BN * 8) continue;
+                    char* d = base + (i < NH ? i * T : BM * 8 + (i - NH) * T) * 16;
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(i < NH ? rH : rW, (__attribute__((address_space(3))) void*)d, 16, at0[i], at, 0, 0);
+                }
+            } else {  // the rows' ends: chunks behind them come from a line of zeros
+#pragma unroll
+                for (int i = 0; i < NH + NW; ++i) {
+                    if (W_PART && i == NH + NW - 1 && (i - NH) * T + wave * 64 >= BN * 8) continue;
+                    const char* p = at + koff[i] < kbytes ? (i < NH ? Ht : Wt) + at0[i] + at : reinterpret_cast<const char*>(g_zeros);
+                    char* d = base + (i < NH ? i * T : BM * 8 + (i - NH) * T) * 16;
+                    __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)d, 16, 0, 0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NH + NW; ++i) {
+                if (W_PART && i == NH + NW - 1 && (i - NH) * T + wave * 64 >= BN * 8) continue;
+                if ((KIND == K_F32 || KIND == K_F32P) && i < NH && !a.H) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) reg[i][x] = at + koff[i] + 4 * x < kbytes ? __builtin_bit_cast(int, a.h_const) : 0;
+                } else if (whole) {
+                    __builtin_memcpy(&reg[i], src[i] + at + koff[i], 16);
                 } else {
-                    h[j] = load_chunk<KIND>(a.H + (int64_t)r * a.ldh * ES, off, kbytes);
+                    reg[i] = load_chunk(src[i], at + koff[i], kbytes);
                 }
             }
-        };
-        load(0);
-        for (int st = 0; st < steps; ++st) {
-            __syncthreads();  // (the last stage's reads are done)
+        }
+    };
+    auto deposit = [&](int buf) {
+        if constexpr (!DIRECT) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int o = (lr + 32 * j) * RB + ((lc ^ (lr & 7)) << 4);
-                *reinterpret_cast<i32x4*>(sH + o) = h[j];
-                *reinterpret_cast<i32x4*>(sW + o) = w[j];
+            for (int i = 0; i < NH + NW; ++i) {
+                if (W_PART && i == NH + NW - 1 && (i - NH) * T + wave * 64 >= BN * 8) continue;
+                const int c = (i < NH ? i * T : BM * 8 + (i - NH) * T) + tid;
+                *reinterpret_cast<i32x4*>(smem + buf * BUF + c * 16) = reg[i];
             }
-            __syncthreads();
-            if (st + 1 < steps) load(st + 1);
+        }
+    };
+
+    Acc acc[TM][TN] = {};
+    constexpr bool AHEAD = WM * WN == 8;
+    i32x4 fh[AHEAD ? 2 : 1][RT], fw[AHEAD ? 2 : 1][TN];
+    auto read_phase = [&](int buf, int p) {
+        const char* sH = smem + buf * BUF;
+        const char* sW = sH + BM * RB;
+        const int k = p / HALVES, half = p % HALVES;
+        if (half == 0) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                i32x4 fh[2], fw[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    fh[j] = lds_frag<KIND, RB>(sH, wm + j * 16 + (lane & 15), k);
-                    fw[j] = lds_frag<KIND, RB>(sW, wn + j * 16 + (lane & 15), k);
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) acc[i][j] = mfma_step<KIND>(fw[j], fh[i], acc[i][j]);
+            for (int j = 0; j < TN; ++j) {
+                const int row = w_row<KIND, TN>(lane & 15, j);
+                fw[AHEAD ? k : 0][j] = lds_frag<KIND, RB>(sW, wn + row, w_key<KIND, TN>(row), k);
             }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < RT; ++i) fh[AHEAD ? p & 1 : 0][i] = lds_frag<KIND, RB>(sH, wm + (half * RT + i) * 16 + (lane & 15), lane & 7, k);
+    };
+    auto multiply_rows = [&](int p, int from, int to) {
+        const int k = p / HALVES, half = p % HALVES;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int r = t.row0 + wm + i * 16 + (lane & 15);
-                if (r >= t.row1) continue;
-                if constexpr (KIND == K_F32P) {
-                    // (the double instruction returns row 4 i + (lane >> 4) in register i)
-                    const int64_t ch = (int64_t)t.model * a.ctot;
+        for (int i = from; i < to; ++i)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const int n = n0 + wn + j * 16 + 4 * x + (lane >> 4);
-                        if (n >= a.ctot) continue;
-                        float v = (float)acc[i][j][x];
-                        if (a.bias) v += a.bias[ch + n];
-                        reinterpret_cast<float*>(a.Y)[(int64_t)r * a.ldy + n] = apply_act(v, a.act);
-                    }
-                } else {
-                    const int n = n0 + wn + j * 16 + 4 * (lane >> 4);
-                    if (n < a.ctot) finish4<KIND>(a, t, r, n, acc[i][j]);
+            for (int j = 0; j < TN; ++j)
+                acc[half * RT + i][j] = mfma_step<KIND>(fw[AHEAD ? k : 0][j], fh[AHEAD ? p & 1 : 0][i], acc[half * RT + i][j]);
+    };
+
+    static_assert(DIRECT || NBUF == 2, "stages that travel through registers are fetched one ahead");
+    static_assert(NBUF == 2 || !W_PART, "every wave has the same loads in flight");
+    fetch(0, 0);
+    if constexpr (DIRECT) {
+        if (NBUF == 3 && steps > 1) {
+            fetch(1, 1);
+            arrive_all<DIRECT, NH + NW>();
+        } else {
+            arrive_all<DIRECT, 0>();
+        }
+        if (steps > NBUF - 1) fetch(NBUF - 1, NBUF - 1);
+    } else {
+        deposit(0);
+        if (steps > 1) fetch(1, 1);
+        arrive_all<DIRECT, 0>();
+    }
+    const int live = a.ctot - n0 <= wn ? 0 : min(HALVES, (t.row1 - t.row0 - wm + RT * 16 - 1) / (RT * 16));  // halves with rows
+    auto run = [&](auto all) {
+        constexpr bool ALL = decltype(all)::value;
+        if (AHEAD && (ALL || live > 0)) read_phase(0, 0);
+        int cur = 0;  // the buffer of stage st
+        for (int st = 0; st < steps; ++st) {
+            const int next = cur + 1 == NBUF ? 0 : cur + 1;
+#pragma unroll
+            for (int p = 0; p < PHASES; ++p) {
+                const bool mine = ALL || p % HALVES < live, last = p + 1 == PHASES;
+                if (mine) {
+                    if (!AHEAD) read_phase(cur, p);
+                    multiply_rows(p, 0, AHEAD ? 1 : RT);
+                }
+                if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
+                if (last && st + 1 < steps) {
+                    // stage st + 1 lies in its buffer, everyone has read all of stage st
+                    deposit(next);
+                    if (NBUF == 3 && st + 2 < steps) arrive_all<DIRECT, NH + NW>();
+                    else arrive_all<DIRECT, 0>();
+                    if (st + NBUF < steps) fetch(st + NBUF, cur);
+                }
+                if constexpr (AHEAD) {
+                    if (!last ? ALL || (p + 1) % HALVES < live : st + 1 < steps && (ALL || live > 0))
+                        read_phase(last ? next : cur, last ? 0 : p + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_s_setprio(1);
+                    if (mine) multiply_rows(p, 1, RT);
+                    __builtin_amdgcn_s_setprio(0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-        __syncthreads();  // (the next tile's first stage overwrites the LDS)
+            cur = next;
+        }
+    };
+    if (live == HALVES) run(std::true_type{});
+    else run(std::false_type{});
+    if (live == 0) return;
+    if constexpr (KIND == K_BF16) write_tiles<KIND, __bf16, TM, TN>(a, t, wm, n0 + wn, acc);
+    else if constexpr (KIND == K_F16) write_tiles<KIND, _Float16, TM, TN>(a, t, wm, n0 + wn, acc);
+    else if constexpr (KIND != K_I8) write_tiles<KIND, float, TM, TN>(a, t, wm, n0 + wn, acc);
+    else if (a.out_dtype == DGCN_BF16) write_tiles<KIND, __bf16, TM, TN>(a, t, wm, n0 + wn, acc);
+    else if (a.out_dtype == DGCN_F16) write_tiles<KIND, _Float16, TM, TN>(a, t, wm, n0 + wn, acc);
+    else write_tiles<KIND, float, TM, TN>(a, t, wm, n0 + wn, acc);
+}
+
+template <int KIND, int BM, int BN, int WM, int WN, int NBUF, bool DIRECT>
+__global__ __launch_bounds__(WM* WN * 64) void k_product(ProductArgs a, int64_t slots, int col_tiles) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    product_tile<KIND, BM, BN, WM, WN, NBUF, DIRECT>(a, slots, col_tiles, smem);
+}
+
+// Few rows per group: the weights' bytes are the cost.  A workgroup takes 16 rows x 16 NT columns; its waves share the k range in
+// interleaved pieces of 128 bytes, read their fragments straight from memory (every weight is used once: LDS would only be a
+// detour) and join their sums through LDS in a fixed order.
+template <int KIND, int NT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void k_product_few(ProductArgs a, int64_t slots, int col_tiles) {
+    constexpr int ES = Elem<KIND>::size, BM = 16, BN = 16 * NT;
+    using Acc = typename Elem<KIND>::Acc;
+    __shared__ __attribute__((aligned(16))) Acc part[WAVES][NT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4;
+    const int64_t kbytes = (int64_t)a.cin * ES;
+    const Tile t = find_tile<BM>(a, blockIdx.x, slots, col_tiles);
+    if (t.row0 >= t.row1) return;
+    const int n0 = t.col * BN;
+    const char* h = a.H + (t.row0 + (int64_t)min(lane & 15, t.row1 - 1 - t.row0)) * a.ldh * ES;
+    const char* w[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+        w[j] = a.W + ((int64_t)t.model * a.ctot + n0 + min(j * 16 + (lane & 15), a.ctot - 1 - n0)) * kbytes;
+    Acc acc[NT] = {};
+    const int pieces = (int)((kbytes + 127) >> 7);
+    // whole pieces; of rows that start anywhere, those that are neither first nor last
+    const int from = a.dwords ? 0 : 1, to = (int)((a.dwords ? kbytes : kbytes - 4) >> 7);
+    constexpr int U = NT >= 4 ? 2 : 4;
+    int c = wave;
+    auto checked = [&](int c) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int64_t off = (int64_t)c * 128 + e * 64 + q * 16;
+            const i32x4 fh = load_chunk(h, off, kbytes);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[j] = mfma_step<KIND>(load_chunk(w[j], off, kbytes), fh, acc[j]);
+        }
+    };
+    auto whole = [&](auto dwords, int c, auto count) {
+        constexpr bool DW = decltype(dwords)::value;
+        constexpr int N = decltype(count)::value;
+        i32x4 fh[N][2], fw[N][2][NT];
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int64_t off = (int64_t)(c + u * WAVES) * 128 + e * 64 + q * 16;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    if constexpr (DW) __builtin_memcpy(&fw[u][e][j], w[j] + off, 16);
+                    else fw[u][e][j] = shift_dwords(load_dwords(w[j] + off), (int)(uintptr_t)w[j] & 3);
+                }
+                if constexpr (DW) __builtin_memcpy(&fh[u][e], h + off, 16);
+                else fh[u][e] = shift_dwords(load_dwords(h + off), (int)(uintptr_t)h & 3);
+            }
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[j] = mfma_step<KIND>(fw[u][e][j], fh[u][e], acc[j]);
+    };
+    if (c < from && c < pieces) {
+        checked(c);
+        c += WAVES;
+    }
+    auto middle = [&](auto dwords) {
+        for (; c + (U - 1) * WAVES < to; c += U * WAVES) whole(dwords, c, std::integral_constant<int, U>{});
+        for (; c < to; c += WAVES) whole(dwords, c, std::integral_constant<int, 1>{});
+    };
+    if (ES == 4 || a.dwords) middle(std::true_type{});
+    else middle(std::false_type{});
+    if (c < pieces) checked(c);  // (one of at most two last pieces)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) part[wave][j][lane] = acc[j];
+    __syncthreads();
+    for (int x = threadIdx.x; x < NT * 64; x += WAVES * 64) {
+        const int j = x >> 6, l = x & 63;
+        Acc sum = part[0][j][l];
+#pragma unroll
+        for (int v = 1; v < WAVES; ++v) sum += part[v][j][l];
+        const int64_t r = (int64_t)t.row0 + (l & 15);
+        const int n = n0 + j * 16 + 4 * (l >> 4);
+        if (r >= t.row1 || n >= a.ctot) continue;
+        float ws[4], bias[4], v[4];
+        column_values<KIND, 4>(a, t.model, n, ws, bias);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (float)sum[i];
+        const float hs = KIND == K_I8 ? a.hs[r] : 0.f;
+        if (a.out_dtype == DGCN_BF16) finish<KIND, __bf16, 4>(a, r, n, v, hs, ws, bias);
+        else if (a.out_dtype == DGCN_F16) finish<KIND, _Float16, 4>(a, r, n, v, hs, ws, bias);
+        else finish<KIND, float, 4>(a, r, n, v, hs, ws, bias);
     }
 }
 
-static size_t dtype_size(int32_t d) { return d == DGCN_F32 ? 4 : 2; }
+// Many rows of a narrow layer (rows of at most KS x 64 bytes, whole 16-byte chunks; at most 16 TN columns): memory-bound, so no LDS and
+// no barrier.  Every wave walks a contiguous run of rows in windows of 16 whose loads need no knowledge of the groups and are in flight
+// one window ahead; the weights of the group it is in are MFMA fragments in registers.  A window that several groups share is multiplied
+// once for each and stored row by row.
+//
+// A lane's 16 bytes of H hold float32 elements 4 q .. 4 q + 3 (q = lane >> 4), the ascending chain needs element 4 s + q in MFMA s: a
+// 4 x 4 transpose between the four lane groups and the four registers, in four lane-swap instructions.
+template <int KIND> __device__ __forceinline__ i32x4 chain_order(i32x4 v) {
+    if constexpr (KIND == K_F32) {
+        auto a = __builtin_amdgcn_permlane32_swap((unsigned)v[0], (unsigned)v[2], false, false);
+        auto b = __builtin_amdgcn_permlane32_swap((unsigned)v[1], (unsigned)v[3], false, false);
+        auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+        auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+        return i32x4{(int)c[0], (int)c[1], (int)d[0], (int)d[1]};
+    } else {
+        return v;
+    }
+}
 
-template <int KIND> static int launch_any(const char* family, const ProductArgs& a, hipStream_t s) {
-    const int64_t slots = a.gptr ? (int64_t)a.rows / 64 + a.num_groups : ((int64_t)a.rows + 63) / 64;
-    const int col_tiles = ceil_div(a.ctot, 64);
-    const int blocks = (int)min(slots * col_tiles, (int64_t)1 << 20);
+template <int KIND, class O, int TN, int KS>
+__device__ __forceinline__ void product_rows(const ProductArgs& a, int run) {
+    constexpr int ES = Elem<KIND>::size;
+    using Acc = typename Elem<KIND>::Acc;
+    const int lane = threadIdx.x & 63, q = lane >> 4;
+    const int64_t kbytes = (int64_t)a.cin * ES;
+    const int64_t gw = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto clamp = [&](int p) { return min(max(p, 0), a.rows); };
+    if (a.gptr) {  // every table entry is checked by one thread
+        for (int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x; g < a.num_groups; g += (int64_t)gridDim.x * 256)
+            if (bad_group(a, a.gptr[g], a.gptr[g + 1], a.mog ? a.mog[g] : (int)g)) atomicOr(a.status, (int)DGCN_FAULT_BAD_GROUP);
+    }
+    int64_t r = gw * run;  // the next row to compute
+    const int64_t end = min(r + run, (int64_t)a.rows);
+    if (r >= end) return;
+    auto load_h = [&](int64_t window, i32x4 (&h)[KS]) {
+        const char* row = a.H + min(window + (lane & 15), (int64_t)a.rows - 1) * a.ldh * ES;
+#pragma unroll
+        for (int e = 0; e < KS; ++e) {
+            h[e] = i32x4{0, 0, 0, 0};
+            if (e * 64 + q * 16 < kbytes) __builtin_memcpy(&h[e], row + e * 64 + q * 16, 16);
+        }
+    };
+    int64_t p0 = 0, p1 = 0;  // the group of row r (none yet)
+    int e = -1, model = -1;
+    auto find_group = [&]() {  // the last group that starts at or in front of row r
+        if (!a.gptr) { p1 = a.rows; e = 0; return; }
+        int lo = 0, n = a.num_groups;
+        while (n > 64) {
+            const int step = (n + 63) >> 6;
+            const int64_t i = (int64_t)lane * step;
+            const unsigned long long m = __ballot(i < n && clamp(a.gptr[lo + (i < n ? (int)i : 0)]) <= r);
+            const int k = max(m == ~0ull ? 64 : (int)__builtin_ctzll(~m), 1);
+            lo += (k - 1) * step;
+            n = min(step, n - (k - 1) * step);
+        }
+        const int g = lo + min(lane, n - 1);
+        const int q0 = clamp(a.gptr[g]), q1 = clamp(a.gptr[g + 1]), qe = a.mog ? a.mog[g] : g;
+        const unsigned long long m = __ballot(lane < n && q0 <= r);
+        const int at = __builtin_amdgcn_readfirstlane(max(m == ~0ull ? 64 : (int)__builtin_ctzll(~m), 1) - 1);
+        p0 = __builtin_amdgcn_readlane(q0, at);
+        p1 = __builtin_amdgcn_readlane(q1, at);
+        e = __builtin_amdgcn_readlane(qe, at);
+        if (r < p0) {  // in front of the first group: rows of no group up to it
+            p1 = p0;
+            e = -1;
+        } else if (r >= p1) {  // behind the last one; in a table that decreases, on by a step
+            p1 = lo + at + 1 == a.num_groups ? end : min(r + 16, end);
+            e = -1;
+        }
+    };
+    i32x4 w[TN][KS];
+    float ws[TN][4], bias[TN][4];
+    i32x4 h[KS], ahead[KS];
+    load_h(r, h);
+    for (int64_t window = r; window < end; window += 16) {
+        const int64_t wend = min(window + 16, end);
+        if (wend < end) load_h(wend, ahead);
+        i32x4 hk[KS];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) hk[k] = chain_order<KIND>(h[k]);
+        while (r < wend) {
+            if (r >= p1) find_group();
+            const int64_t stop = min(p1, wend);
+            if (e >= 0 && e < a.num_models) {
+                if (e != model) {
+                    model = e;
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) {
+                        const char* row = a.W + ((int64_t)e * a.ctot + min(w_row<KIND, TN>(lane & 15, j), a.ctot - 1)) * kbytes;
+#pragma unroll
+                        for (int k = 0; k < KS; ++k) {
+                            w[j][k] = i32x4{0, 0, 0, 0};
+                            if (k * 64 + q * 16 < kbytes) __builtin_memcpy(&w[j][k], row + k * 64 + q * 16, 16);
+                            w[j][k] = chain_order<KIND>(w[j][k]);
+                        }
+                        column_values<KIND, 4>(a, e, min(w_row<KIND, TN>(4 * q, j), a.ctot - 1), ws[j], bias[j]);
+                    }
+                }
+                Acc acc[TN] = {};
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) acc[j] = mfma_step<KIND>(w[j][k], hk[k], acc[j]);
+                const int64_t row = window + (lane & 15);
+                if (row >= r && row < stop) {
+                    const float hs = KIND == K_I8 ? a.hs[row] : 0.f;
+                    constexpr int PW = TN % 2 == 0 ? 2 : 1, CH = 4 * PW;
+#pragma unroll
+                    for (int p = 0; p < TN / PW; ++p) {
+                        const int n = p * 16 * PW + q * CH;
+                        float v[CH], s[CH], b[CH];
+#pragma unroll
+                        for (int x = 0; x < CH; ++x) {
+                            v[x] = (float)acc[p * PW + (x >> 2)][x & 3];
+                            s[x] = ws[p * PW + (x >> 2)][x & 3];
+                            b[x] = bias[p * PW + (x >> 2)][x & 3];
+                        }
+                        if (n < a.ctot) finish<KIND, O, CH>(a, row, n, v, hs, s, b);
+                    }
+                }
+            }
+            r = stop;
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k) h[k] = ahead[k];
+    }
+}
+
+template <int KIND, class O, int TN, int KS>
+__global__ __launch_bounds__(256) void k_product_rows(ProductArgs a, int run) { product_rows<KIND, O, TN, KS>(a, run); }
+
+static int64_t row_slots(const ProductArgs& a, int BM) {
+    if (!a.gptr) return ((int64_t)a.rows + BM - 1) / BM;
+    const int64_t n = (int64_t)a.rows / BM + a.num_groups;
+    return a.num_groups <= kCountedGroups ? min(n, (int64_t)a.rows) : n;  // (a counted tile holds at least one row)
+}
+constexpr int64_t max_grid(int threads) { return 0xffffffffu / (unsigned)threads; }  // a launch's threads are counted in 32 bits
+
+template <int KIND, int BM, int BN, int WM, int WN, int NBUF, bool DIRECT>
+static int launch_tiles_as(const char* family, const ProductArgs& a, hipStream_t s) {
+    const int64_t slots = row_slots(a, BM);
+    const int col_tiles = (a.ctot + BN - 1) / BN;
+    if (slots * col_tiles > max_grid(WM * WN * 64)) return fail(DGCN_ERR_UNSUPPORTED, "%s: %lld tiles in one call", family, (long long)(slots * col_tiles));
+    const int lds = (int)min(((int64_t)a.cin * Elem<KIND>::size - 1) / kRowBytes + 1, (int64_t)NBUF) * (BM + BN) * kRowBytes;
+    if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product<KIND, BM, BN, WM, WN, NBUF, DIRECT>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, NBUF * (BM + BN) * kRowBytes) != hipSuccess)
+        return fail(DGCN_ERR_LAUNCH, "%s: %d bytes of LDS are not available", family, lds);
     TimedLaunch t(family, s);
-    DGCN_LAUNCH(t, (k_product_any<KIND>), dim3(blocks), dim3(256), 0, s, a, slots, col_tiles);
-    return check_launch("k_product_any");
+    DGCN_LAUNCH(t, (k_product<KIND, BM, BN, WM, WN, NBUF, DIRECT>), dim3((unsigned)(slots * col_tiles)), dim3(WM * WN * 64), lds, s, a, slots, col_tiles);
+    return check_launch("k_product");
+}
+
+// Load-to-LDS instructions take rows at 16-byte strides; a tile's offsets are 31 bits.
+template <int KIND> static bool direct_loads(const ProductArgs& a) {
+    constexpr int64_t ES = Elem<KIND>::size;
+    return a.H && ((uintptr_t)a.H | (uintptr_t)a.W) % 16 == 0 && a.ldh * ES % 16 == 0 && a.cin * ES % 16 == 0 && a.ldh * ES * 256 < 0x7fffffff &&
+           a.cin * ES * 256 < 0x7fffffff;
+}
+
+template <int KIND, int BM, int BN, int WM, int WN, int NBUF>
+static int launch_tiles(const char* family, const ProductArgs& a, hipStream_t s) {
+    if (direct_loads<KIND>(a)) return launch_tiles_as<KIND, BM, BN, WM, WN, NBUF, true>(family, a, s);
+    return launch_tiles_as<KIND, BM, BN, WM, WN, 2, false>(family, a, s);
+}
+
+template <int KIND, int NT, int WAVES> static int launch_few(const char* family, const ProductArgs& a, hipStream_t s) {
+    const int64_t slots = row_slots(a, 16);
+    const int col_tiles = (a.ctot + 16 * NT - 1) / (16 * NT);
+    if (slots * col_tiles > max_grid(WAVES * 64)) return fail(DGCN_ERR_UNSUPPORTED, "%s: %lld tiles in one call", family, (long long)(slots * col_tiles));
+    TimedLaunch t(family, s);
+    DGCN_LAUNCH(t, (k_product_few<KIND, NT, WAVES>), dim3((unsigned)(slots * col_tiles)), dim3(WAVES * 64), 0, s, a, slots, col_tiles);
+    return check_launch("k_product_few");
+}
+
+template <int KIND, class O, int TN, int KS> static int launch_rows_as(const char* family, const ProductArgs& a, hipStream_t s) {
+    constexpr int waves = kCUs * 24;
+    const int64_t tiles = ((int64_t)a.rows + 15) / 16;
+    const int run = (int)((tiles + waves - 1) / waves) * 16;
+    const int64_t blocks = ((int64_t)a.rows + 4 * (int64_t)run - 1) / (4 * (int64_t)run);
+    TimedLaunch t(family, s);
+    DGCN_LAUNCH(t, (k_product_rows<KIND, O, TN, KS>), dim3((unsigned)blocks), dim3(256), 0, s, a, run);
+    return check_launch("k_product_rows");
+}
+template <int KIND, int TN, int KS> static int launch_rows(const char* family, const ProductArgs& a, hipStream_t s) {
+    if constexpr (KIND == K_F32) return launch_rows_as<KIND, float, TN, KS>(family, a, s);
+    else if constexpr (KIND == K_BF16) return launch_rows_as<KIND, __bf16, TN, KS>(family, a, s);
+    else if constexpr (KIND == K_F16) return launch_rows_as<KIND, _Float16, TN, KS>(family, a, s);
+    else if (a.out_dtype == DGCN_F32) return launch_rows_as<KIND, float, TN, KS>(family, a, s);
+    else if (a.out_dtype == DGCN_BF16) return launch_rows_as<KIND, __bf16, TN, KS>(family, a, s);
+    else return launch_rows_as<KIND, _Float16, TN, KS>(family, a, s);
+}
+
+// The tile shapes of the 8- and 16-bit products and what they cost, fitted to 26 shapes of 128 .. 100 000 rows, k of 64 .. 4 096 bytes and
+// 20 .. 4 096 columns, dense and in 8 .. 300 groups: a stage (128 bytes of k) takes s1 us in a workgroup that has its CU to itself and sc
+// us with per_cu of them there, a tile's start and end f us.  The least estimate is the fastest shape or within 14 % of it on 22 of the
+// 26 (the others: many groups of few rows, up to 35 %).
+struct Shape { int bm, bn, per_cu; float s1, sc, f; };
+constexpr int kShapes = 5;
+constexpr Shape kDirect[kShapes] = {{64, 64, 5, .55f, 1.11f, 2.f}, {128, 128, 2, .78f, 1.05f, 3.f}, {128, 256, 1, .98f, .98f, 4.f},
+                                    {192, 256, 1, 1.36f, 1.36f, 5.f}, {256, 256, 1, 1.8f, 1.8f, 6.f}};
+constexpr Shape kStaged[kShapes] = {{64, 64, 4, .85f, 1.6f, 2.f}, {128, 128, 1, 1.23f, 1.23f, 3.f}, {128, 256, 1, 1.7f, 1.7f, 4.f},
+                                    {192, 256, 1, 2.05f, 2.05f, 5.f}, {0, 0, 0, 0.f, 0.f, 0.f}};
+
+// Row tiles a launch is expected to have: the host knows rows and groups, not the groups' sizes.
+static float expected_slots(const ProductArgs& a, int BM) {
+    if (!a.gptr) return (float)(((int64_t)a.rows + BM - 1) / BM);
+    return (float)a.rows / BM + .5f * min(a.num_groups, a.rows);
+}
+
+static int choose_shape(const ProductArgs& a, int64_t row_bytes, bool direct) {
+    const Shape* shapes = direct ? kDirect : kStaged;
+    const float steps = (float)((row_bytes + kRowBytes - 1) / kRowBytes);
+    int best = 0;
+    float least = INFINITY;
+    for (int i = 0; i < kShapes; ++i) {
+        const Shape& p = shapes[i];
+        if (!p.bm) continue;
+        const float per = expected_slots(a, p.bm) * (float)((a.ctot + p.bn - 1) / p.bn) / kCUs;  // tiles per CU
+        const float rounds = floorf(per / p.per_cu), rest = per - rounds * p.per_cu;
+        float cost = rounds * (p.sc * steps + p.f);
+        if (rest > .02f) cost += (p.s1 + (p.per_cu > 1 ? (p.sc - p.s1) * (ceilf(rest) - 1.f) / (p.per_cu - 1) : 0.f)) * steps + p.f;
+        if (cost < least) { least = cost; best = i; }
+    }
+    // Groups of so few rows that the weights are nearly all the bytes, and those bytes are the time: 128 x 128 reads them once more seldom
+    // (64 groups, 2 048 rows, 2 048 bytes x 1 024 columns: 27.8 us against 37.5 of the 64 x 64 tile).
+    const float weights = (float)min(a.num_groups, a.rows) * a.ctot * row_bytes, rest = (float)a.rows * (row_bytes + 2.f * a.ctot);
+    if (direct && a.gptr && weights > 4.f * rest && weights / 4.7e6f > least) best = 1;
+    return best;
+}
+
+template <int KIND> static int dispatch_kind(const char* family, const ProductArgs& a, hipStream_t s) {
+    const int64_t row_bytes = (int64_t)a.cin * Elem<KIND>::size;
+    if constexpr (KIND == K_F32P) {
+        return launch_tiles<KIND, 64, 64, 2, 2, 2>(family, a, s);
+    } else {
+        // a narrow layer over very many rows: no tile would be more than a copy (800 000 rows of 32 float32 -> 2: 28 us against 32 of the
+        // 128 x 16 tile; 300 000 rows of 32 bf16 -> 32: 12 against 19 of 64 x 64; at 60 000 rows no difference)
+        if (a.H && a.dwords && row_bytes % 16 == 0 && row_bytes <= 128 && a.ctot <= 32 && a.rows >= 1 << 17)
+            return a.ctot <= 16 ? launch_rows<KIND, 1, 2>(family, a, s) : launch_rows<KIND, 2, 2>(family, a, s);
+    }
+    const int groups = min(a.num_groups, a.rows);
+    if constexpr (KIND == K_F32) {
+        // float32: the matrix pipe is the bound from some 64 columns on, so the shape matters little but for its waste.  128 x 128 (1 024
+        // x 1 024, 8 192 rows: 144 us against 165) where its tiles fill whole rounds of two per CU; 64 x 64 where a row is one stage (32
+        // -> 64, 500 graphs: 16.4 against 19.4 of 32 x 64), else 32 x 64 (128 -> 256: 96 against 101; 200 rows in 10 groups: 12 against 15).
+        const float rounds = expected_slots(a, 128) * (float)((a.ctot + 127) / 128) / (2 * kCUs);
+        if (a.ctot <= 16) return launch_tiles<KIND, 128, 16, 4, 1, 2>(family, a, s);
+        if (a.ctot <= 32 && row_bytes > 128) return launch_tiles<KIND, 128, 32, 4, 1, 2>(family, a, s);
+        if (groups == 1 && row_bytes >= 1024 && rounds > .9f * ceilf(rounds)) return launch_tiles<KIND, 128, 128, 2, 4, 2>(family, a, s);
+        if (row_bytes <= 128 && a.rows / groups >= 48) return launch_tiles<KIND, 64, 64, 2, 2, 2>(family, a, s);
+        return launch_tiles<KIND, 32, 64, 1, 4, 2>(family, a, s);
+    } else if constexpr (KIND != K_F32P) {
+        // few rows in every group, long rows and not enough tiles to fill the chip: split k over a workgroup's waves (1 row, 4 096 x
+        // 4 096 int8: 6 us against 17 of the 64 x 64 tile; 64 rows: 15 against 19; 24 rows in 64 groups, fp16 2 048 x 1 024: 23 against 29)
+        const int64_t tiles = (a.gptr ? (int64_t)groups : (a.rows + 63) / 64) * ((a.ctot + 63) / 64);
+        if (row_bytes >= 512 && a.rows <= (a.gptr ? 16 * (int64_t)groups : 64) && tiles < 2 * kCUs) {
+            if (a.gptr || a.rows > 16) return launch_few<KIND, 2, 4>(family, a, s);
+            return row_bytes >= 2048 ? launch_few<KIND, 1, 8>(family, a, s) : launch_few<KIND, 1, 4>(family, a, s);
+        }
+        const bool direct = direct_loads<KIND>(a);
+        switch (choose_shape(a, row_bytes, direct)) {
+            case 0: return launch_tiles<KIND, 64, 64, 2, 2, 2>(family, a, s);
+            case 1: return launch_tiles<KIND, 128, 128, 2, 4, 2>(family, a, s);
+            case 2: return launch_tiles<KIND, 128, 256, 2, 4, 3>(family, a, s);
+            case 3: return launch_tiles<KIND, 192, 256, 2, 4, 2>(family, a, s);
+            default: return launch_tiles_as<KIND, 256, 256, 2, 4, 2, true>(family, a, s);
+        }
+    }
 }
 
 static int product_dispatch(const char* family, int kind, ProductArgs& a, hipStream_t s) {
-    const size_t os = dtype_size(a.out_dtype);
-    a.vec_out = a.ldy % 4 == 0 && (uintptr_t)a.Y % (4 * os) == 0;
+    const int es = kind == K_I8 ? 1 : kind == K_BF16 || kind == K_F16 ? 2 : 4;
+    a.dwords = es == 4 || (((uintptr_t)a.H | (uintptr_t)a.W) % 4 == 0 && a.ldh * es % 4 == 0 && (int64_t)a.cin * es % 4 == 0);
     switch (kind) {
-        case K_I8: return launch_any<K_I8>(family, a, s);
-        case K_BF16: return launch_any<K_BF16>(family, a, s);
-        case K_F16: return launch_any<K_F16>(family, a, s);
-        case K_F32: return launch_any<K_F32>(family, a, s);
-        default: return launch_any<K_F32P>(family, a, s);
+        case K_I8: return dispatch_kind<K_I8>(family, a, s);
+        case K_BF16: return dispatch_kind<K_BF16>(family, a, s);
+        case K_F16: return dispatch_kind<K_F16>(family, a, s);
+        case K_F32: return dispatch_kind<K_F32>(family, a, s);
+        default: return dispatch_kind<K_F32P>(family, a, s);
     }
 }
 

@@ -142,6 +142,63 @@ def test_transform_int8(engine, rows, cin, ctot, dtype):
         assert torch.equal(engine.transform_int8(h, hs, w[0], ws[0], bias=bias[0] if use_bias else None, act=act, dtype=buf.dtype), y)
 
 
+# one entry per tile shape and loader of the 8- and 16-bit products, per kernel for few rows, and their neighbours (an odd row, column, depth)
+@pytest.mark.parametrize("rows,cin,ctot", [(8192, 4096, 4096), (8191, 4095, 4097), (4096, 2048, 2048), (4097, 2047, 2050), (9000, 1024, 2000), (8800, 1000, 2001),
+                                            (100000, 512, 512), (60001, 300, 65), (1024, 4096, 4096), (1, 4096, 4096), (16, 4095, 513), (17, 2048, 700),
+                                            (64, 1024, 1024), (33, 1030, 40), (200000, 128, 16), (140001, 96, 30), (131072, 64, 5)])
+def test_transform_int8_large(engine, rows, cin, ctot):
+    h, w, hs, ws, bias = _int8_inputs(rows, cin, ctot, 1, rows + cin)
+    _check_int8(engine.transform_int8(h, hs, w[0], ws[0], bias=bias[0], act="leaky_relu"), h, w[0], hs, ws[0], bias[0], "leaky_relu", "float32")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("rows,cin,ctot,groups", [(8192, 2048, 4096, 8), (8191, 2047, 2049, 8), (8192, 2048, 4096, 1), (2048, 1024, 1024, 64), (24, 2048, 1024, 64),
+                                                   (24, 2047, 1000, 64), (5, 777, 90, 300), (300000, 32, 32, 2000), (200000, 64, 7, 300), (150000, 48, 20, 1),
+                                                   (3000, 500, 500, 257), (20000, 200, 120, 256)])
+def test_grouped_half_precision_large(engine, rows, cin, ctot, groups, dtype):
+    """Uneven groups (some empty); every group its own weights, or one of eight models."""
+    import torch
+    rng = np.random.default_rng(rows)
+    cut = np.sort(rng.integers(0, rows + 1, groups - 1)) if groups > 1 else np.zeros(0, int)
+    sizes = np.diff(np.concatenate([[0], cut, [rows]])).tolist()
+    ptr, blocks = _groups(sizes)
+    M = groups if groups <= 64 else 8
+    of = [g if groups <= 64 else int(rng.integers(0, M)) for g in range(groups)]
+    g, t = _gen(cin), getattr(torch, dtype)
+    H = torch.randn(rows, cin, device="cuda:0", generator=g).to(t)
+    W = torch.randn(M, ctot, cin, device="cuda:0", generator=g).to(t)
+    y = engine.transform_grouped(H, W, ptr, model_of_group=None if groups <= 64 else torch.tensor(of, dtype=torch.int32, device="cuda:0"))
+    of_row = torch.repeat_interleave(torch.tensor(of), torch.tensor(sizes)).cuda()
+    for m in range(M):
+        idx = torch.nonzero(of_row == m).flatten()
+        if idx.numel() == 0:
+            continue
+        h, w = H[idx].double(), W[m].double()
+        want, mag = h @ w.t(), h.abs() @ w.abs().t()
+        tol = 2.01 * U * cin * mag
+        tol = tol + HALF_STEP[dtype] * (want.abs() + tol) + SUBNORMAL[dtype]
+        assert bool(((y[idx].double() - want).abs() <= tol).all()), m
+
+
+@pytest.mark.parametrize("rows,cin,ctot,groups", [(8192, 256, 1024, 1), (8191, 257, 1023, 1), (800000, 32, 2, 4000), (140000, 16, 32, 300), (131072, 8, 17, 257), (50000, 100, 20, 250),
+                                                   (16, 1024, 600, 16), (1, 4096, 33, 1), (300, 31, 65, 7)])
+def test_grouped_float32_large(engine, rows, cin, ctot, groups):
+    import torch
+    rng = np.random.default_rng(rows)
+    cut = np.sort(rng.integers(0, rows + 1, groups - 1)) if groups > 1 else np.zeros(0, int)
+    sizes = np.diff(np.concatenate([[0], cut, [rows]])).tolist()
+    ptr, blocks = _groups(sizes)
+    of = [int(x) for x in rng.integers(0, 3, groups)]
+    H = torch.randn(rows, cin, device="cuda:0", generator=_gen(cin))
+    W = torch.randn(3, ctot, cin, device="cuda:0", generator=_gen(1))
+    of_row = torch.repeat_interleave(torch.tensor(of), torch.tensor(sizes)).cuda()
+    for precise in (False, True):
+        y = engine.transform_grouped(H, W, ptr, model_of_group=torch.tensor(of, dtype=torch.int32, device="cuda:0"), precise=precise)
+        for m in range(3):
+            full = engine.transform(H, W[m].t().contiguous(), precise=precise)
+            assert torch.equal(y[of_row == m], full[of_row == m])
+
+
 def test_int8_sums_are_exact_at_the_largest_depth(engine):
     import torch
     rows, cin, ctot = 3, 131071, 5
