@@ -6,6 +6,7 @@
 // Every type runs the same tile loop in BYTES: 64 bytes of a row of H and of W feed one step of a 16 x 16 output tile, 16 bytes per
 // lane (lane & 15 = the row, lane >> 4 = which 16 of the 64 bytes): one MFMA of int8 (k = 64), bf16 / fp16 (k = 32), four of float32
 // (k = 4 each).  W is the MFMA's A operand and H its B operand, so a lane ends with four output columns n of ONE row r.
+#include <atomic>
 #include <type_traits>
 
 #include "common.h"
@@ -33,7 +34,7 @@ struct ProductArgs {
     int64_t ldh, ldy;    // elements
     float h_const;
     int rows, cin, ctot, num_groups, num_models, act, out_dtype;
-    bool dwords;         // rows of H and W start at multiples of 4 bytes
+    bool dwords_h, dwords_w;  // rows of H, of W start at multiples of 4 bytes
 };
 
 template <int KIND> struct Elem;
@@ -46,21 +47,20 @@ template <> struct Elem<K_F32P> { static constexpr int size = 4; using Acc = f64
 struct Tile { int row0, row1, model, col; };  // rows [row0, row1), columns from col on; row0 >= row1: nothing to do
 
 // Workgroups go to the XCDs round robin; tile numbers are dealt so that an XCD's workgroups take neighbouring tiles (shared rows of
-// H and W meet in its L2).
-__device__ __forceinline__ int64_t xcd_order(int64_t b, int64_t total) {
-    const int64_t q = total >> 3, r = total & 7, x = b & 7;
+// H and W meet in its L2).  (A launch has fewer than 2^24 workgroups: tile numbers and their divisions are 32 bits wide.)
+__device__ __forceinline__ int xcd_order(int b, int total) {
+    const int q = total >> 3, r = total & 7, x = b & 7;
     return x * q + min(x, r) + (b >> 3);
 }
 
-// Tile number b of slots x col_tiles -> slot; `col` <- column tile.  Four slots side by side, column by column: a square-ish patch is in
-// flight at a time.
-__device__ __forceinline__ int64_t patch_order(int64_t b, int64_t slots, int col_tiles, int& col) {
-    const int64_t tile = xcd_order(b, slots * col_tiles);
+// Tile number `tile` of slots x col_tiles -> slot; `col` <- column tile.  Four slots side by side, column by column: a square-ish patch is
+// in flight at a time.
+__device__ __forceinline__ int patch_order(int tile, int slots, int col_tiles, int& col) {
     if (col_tiles == 1) { col = 0; return tile; }
-    const int64_t first = tile / (4 * (int64_t)col_tiles) * 4;
-    const int h = (int)min((int64_t)4, slots - first), in = (int)(tile - first * col_tiles);
-    col = in / h;
-    return first + in % h;
+    const int first = (int)((unsigned)tile / (4u * (unsigned)col_tiles)) * 4;
+    const unsigned h = (unsigned)min(4, slots - first), in = (unsigned)(tile - first * col_tiles);
+    col = (int)(in / h);
+    return first + (int)(in % h);
 }
 
 __device__ __forceinline__ bool bad_group(const ProductArgs& a, int p0, int p1, int e) {
@@ -68,15 +68,16 @@ __device__ __forceinline__ bool bad_group(const ProductArgs& a, int p0, int p1, 
 }
 
 // Up to 256 groups: every wave reads the whole table, four groups per lane, and counts their row tiles, so that every workgroup up to
-// the number of tiles has one (at most min(rows, floor(rows / BM) + num_groups) x column tiles) and the XCDs' shares are equal.  Whole
-// tiles come first, the groups' shorter last tiles behind them: those fill the launch's last round.  Workgroup 0 reports bad entries.
-// Pointers are clamped to [0, rows] before use: a bad table cannot lead out of the matrix.
+// the number of tiles has one (at most min(rows, floor(rows / BM) + num_groups) x column tiles) and the XCDs' shares are equal.  A
+// group's tiles are neighbours, column by column: its weights are read into an XCD's L2 once (64 groups of 256 rows on average, int8
+// 2 000 x 2 050: with the groups' last, shorter tiles numbered behind all others 654 MB passed the L2 instead of 448).  Workgroup 0
+// reports bad entries.  Pointers are clamped to [0, rows] before use: a bad table cannot lead out of the matrix.
 constexpr int kCountedGroups = 256;
-template <int BM> __device__ __forceinline__ Tile find_tile_counted(const ProductArgs& a, int64_t b, int col_tiles) {
+template <int BM> __device__ __forceinline__ Tile find_tile_counted(const ProductArgs& a, int b, int col_tiles) {
     constexpr int N = kCountedGroups / 64;
     const int lane = threadIdx.x & 63;
     const int per = (a.num_groups + 63) >> 6;
-    int p[N], len[N], e[N], whole = 0, part = 0;
+    int p[N], len[N], e[N], sum = 0;
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -90,39 +91,37 @@ template <int BM> __device__ __forceinline__ Tile find_tile_counted(const Produc
             p[i] = min(max(v0, 0), a.rows);
             len[i] = max(min(max(v1, 0), a.rows) - p[i], 0);
         }
-        whole += len[i] / BM;
-        part += len[i] % BM != 0;
+        sum += (int)((unsigned)(len[i] + BM - 1) / BM);
     }
     if (b == 0 && bad) atomicOr(a.status, (int)DGCN_FAULT_BAD_GROUP);
-    int whole_upto = whole, part_upto = part;  // this lane's and all before
+    int upto = sum;  // row tiles of this lane's groups and of all before
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int w = __shfl_up(whole_upto, d), q = __shfl_up(part_upto, d);
-        if (lane >= d) { whole_upto += w; part_upto += q; }
+        const int w = __shfl_up(upto, d);
+        if (lane >= d) upto += w;
     }
-    const int64_t all_whole = __builtin_amdgcn_readlane(whole_upto, 63), all_part = __builtin_amdgcn_readlane(part_upto, 63);
     Tile t{0, 0, 0, 0};
-    const bool in_whole = b < all_whole * col_tiles;
-    if (!in_whole) b -= all_whole * col_tiles;
-    if (!in_whole && b >= all_part * col_tiles) return t;
-    const int slot = (int)patch_order(b, in_whole ? all_whole : all_part, col_tiles, t.col);
-    const int upto = in_whole ? whole_upto : part_upto;
-    const int owner = __builtin_ctzll(__ballot(upto > slot));
-    int at = slot - (upto - (in_whole ? whole : part)), q0 = 0, q1 = 0, qe = -1;  // (meant for the owner: which of its tiles)
+    const int slots = __builtin_amdgcn_readlane(upto, 63);
+    if (b >= (int64_t)slots * col_tiles) return t;  // (a table that goes back and forth counts rows twice: the product may be large)
+    const int tile = xcd_order(b, slots * col_tiles);
+    const int slot = (int)((unsigned)tile / (unsigned)col_tiles);  // (in the order of groups: says which group, not yet which of its tiles)
+    const unsigned long long m = __ballot(upto > slot);
+    if (m == 0) return t;
+    const int owner = __builtin_ctzll(m);
+    int base = upto - sum, q0 = 0, qn = 0, qe = -1, qb = 0;  // the owner's group with that slot: first row, rows, model, first slot
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int n = in_whole ? len[i] / BM : len[i] % BM != 0;
-        if (at >= 0 && at < n) {
-            q0 = p[i] + (in_whole ? at : len[i] / BM) * BM;
-            q1 = min(q0 + BM, p[i] + len[i]);
-            qe = e[i];
-        }
-        at -= n;
+        const int n = (int)((unsigned)(len[i] + BM - 1) / BM);
+        if (slot >= base && slot < base + n) { q0 = p[i]; qn = len[i]; qe = e[i]; qb = base; }
+        base += n;
     }
-    q0 = __builtin_amdgcn_readlane(q0, owner); q1 = __builtin_amdgcn_readlane(q1, owner); qe = __builtin_amdgcn_readlane(qe, owner);
+    q0 = __builtin_amdgcn_readlane(q0, owner); qn = __builtin_amdgcn_readlane(qn, owner);
+    qe = __builtin_amdgcn_readlane(qe, owner); qb = __builtin_amdgcn_readlane(qb, owner);
     if (qe < 0 || qe >= a.num_models) return t;
-    t.row0 = q0;
-    t.row1 = q1;
+    const int tiles = (int)((unsigned)(qn + BM - 1) / BM), at = patch_order(tile - qb * col_tiles, tiles, col_tiles, t.col);
+    if ((unsigned)at >= (unsigned)tiles || (unsigned)t.col >= (unsigned)col_tiles) return t;  // (such a table only)
+    t.row0 = q0 + at * BM;
+    t.row1 = min(t.row0 + BM, q0 + qn);
     t.model = qe;
     return t;
 }
@@ -130,27 +129,26 @@ template <int BM> __device__ __forceinline__ Tile find_tile_counted(const Produc
 // More groups: no count at all.  Group g's row tiles start at slot floor(p_g / BM) + g, which is increasing in g, and
 // ceil((p_{g+1} - p_g) / BM) never exceeds the distance to the next group's start.  So floor(rows / BM) + num_groups slots cover every
 // tile (some slots are empty), and a slot finds its group by search: 64-ary, a lane per probe.  Slot g < num_groups checks entry g.
-template <int BM> __device__ __forceinline__ Tile find_tile(const ProductArgs& a, int64_t b, int64_t slots, int col_tiles) {
+template <int BM> __device__ __forceinline__ Tile find_tile(const ProductArgs& a, int b, int slots, int col_tiles) {
     if (a.gptr && a.num_groups <= kCountedGroups) return find_tile_counted<BM>(a, b, col_tiles);
     Tile t{0, 0, 0, 0};
-    const int64_t slot = patch_order(b, slots, col_tiles, t.col);
+    const int slot = patch_order(xcd_order(b, slots * col_tiles), slots, col_tiles, t.col);
     if (!a.gptr) {
-        t.row0 = (int)(slot * BM);
-        t.row1 = (int)min(slot * BM + BM, (int64_t)a.rows);
+        t.row0 = slot * BM;
+        t.row1 = min(t.row0 + BM, a.rows);
         return t;
     }
     if (t.col == 0 && slot < a.num_groups && threadIdx.x == 0) {
-        const int g = (int)slot;
-        if (bad_group(a, a.gptr[g], a.gptr[g + 1], a.mog ? a.mog[g] : g)) atomicOr(a.status, (int)DGCN_FAULT_BAD_GROUP);
+        if (bad_group(a, a.gptr[slot], a.gptr[slot + 1], a.mog ? a.mog[slot] : slot)) atomicOr(a.status, (int)DGCN_FAULT_BAD_GROUP);
     }
     const int lane = threadIdx.x & 63;
+    auto start = [&](int g, int p) { return (int)((unsigned)p / BM) + g; };  // (below 2^24 for every group of a launch)
     auto clamp = [&](int p) { return min(max(p, 0), a.rows); };
     int lo = 0, n = a.num_groups;  // the group is in [lo, lo + n)
     while (n > 64) {
         const int step = (n + 63) >> 6;
-        const int64_t i = (int64_t)lane * step;
-        const bool below = i < n && (int64_t)(clamp(a.gptr[lo + (i < n ? (int)i : 0)]) / BM) + lo + i <= slot;
-        const unsigned long long m = __ballot(below);
+        const int i = min(lane * step, n - 1);
+        const unsigned long long m = __ballot(lane * step < n && start(lo + i, clamp(a.gptr[lo + i])) <= slot);
         const int k = m == ~0ull ? 64 : __builtin_ctzll(~m);
         if (k == 0) return t;  // in front of the first group
         const int at = (k - 1) * step;
@@ -160,12 +158,12 @@ template <int BM> __device__ __forceinline__ Tile find_tile(const ProductArgs& a
     // at most 64 candidates: a lane each, its pointers and model number with it
     const int g = lo + min(lane, n - 1);
     const int p0 = clamp(a.gptr[g]), p1 = clamp(a.gptr[g + 1]), e = a.mog ? a.mog[g] : g;
-    const unsigned long long m = __ballot(lane < n && (int64_t)(p0 / BM) + g <= slot);
+    const unsigned long long m = __ballot(lane < n && start(g, p0) <= slot);
     const int k = m == ~0ull ? 64 : __builtin_ctzll(~m);
     if (k == 0) return t;
     const int at = __builtin_amdgcn_readfirstlane(k - 1);
     const int q0 = __builtin_amdgcn_readlane(p0, at), q1 = __builtin_amdgcn_readlane(p1, at), qe = __builtin_amdgcn_readlane(e, at);
-    const int64_t r = q0 + (slot - (q0 / BM + (int64_t)lo + at)) * BM;
+    const int64_t r = q0 + (int64_t)(slot - start(lo + at, q0)) * BM;
     if (r < q0 || r >= q1 || qe < 0 || qe >= a.num_models) return t;
     t.row0 = (int)r;
     t.row1 = (int)min(r + BM, (int64_t)q1);
@@ -210,16 +208,20 @@ __device__ __forceinline__ void finish(const ProductArgs& a, int64_t r, int n, c
                                        const float (&bias)[CH]) {
     using V = __attribute__((ext_vector_type(CH))) O;
     V o;
-    const bool relu = a.act == DGCN_ACT_RELU;
-    const float slope = a.act == DGCN_ACT_LEAKY_RELU ? kLeakyAlpha : 1.f;
+    float x[CH];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-        float x = v[i];
-        if constexpr (KIND == K_I8) x = (x * hs) * ws[i];
-        x += bias[i];
-        x = x > 0.f ? x : relu ? 0.f : x * slope;
-        o[i] = (O)x;
+    for (int i = 0; i < CH; ++i) x[i] = KIND == K_I8 ? (v[i] * hs) * ws[i] : v[i];
+    if (a.bias || a.act != DGCN_ACT_LINEAR) {
+        const bool relu = a.act == DGCN_ACT_RELU;
+        const float slope = a.act == DGCN_ACT_LEAKY_RELU ? kLeakyAlpha : 1.f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            x[i] += bias[i];
+            x[i] = x[i] > 0.f ? x[i] : relu ? 0.f : x[i] * slope;
+        }
     }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) o[i] = (O)x[i];
     O* y = reinterpret_cast<O*>(a.Y) + r * a.ldy + n;
     if (n + CH <= a.ctot) {
         __builtin_memcpy(y, &o, sizeof(o));
@@ -344,7 +346,7 @@ constexpr int kRowBytes = 128;  // bytes of k per stage and row
 // fragments are requested behind the first MFMAs of the phase in front of it, across the stage's barrier too, so the matrix pipe
 // does not wait for LDS; smaller tiles have more waves to hide that.  Row tiles behind the group's last row are skipped four at a time.
 template <int KIND, int BM, int BN, int WM, int WN, int NBUF, bool DIRECT>
-__device__ __forceinline__ void product_tile(const ProductArgs& a, int64_t slots, int col_tiles, char* smem) {
+__device__ __forceinline__ void product_tile(const ProductArgs& a, int slots, int col_tiles, char* smem) {
     constexpr int T = WM * WN * 64, RB = kRowBytes, ES = Elem<KIND>::size;
     constexpr int TM = BM / WM / 16, TN = BN / WN / 16;       // 16 x 16 tiles per wave
     constexpr int NH = BM * 8 / T, NW = (BN * 8 + T - 1) / T;  // chunks per thread and stage
@@ -358,7 +360,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int64_t slots
     const int64_t kbytes = (int64_t)a.cin * ES;
     const int steps = (int)((kbytes + RB - 1) / RB);
 
-    const Tile t = find_tile<BM>(a, blockIdx.x, slots, col_tiles);
+    const Tile t = find_tile<BM>(a, (int)blockIdx.x, slots, col_tiles);
     if (t.row0 >= t.row1) return;
     const int n0 = t.col * BN;
     const char* Wm = a.W + (int64_t)t.model * a.ctot * kbytes;
@@ -374,9 +376,10 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int64_t slots
         const bool is_h = i < NH;
         const int c = (is_h ? i : i - NH) * T + tid, row = c >> 3;
         koff[i] = ((c & 7) ^ (is_h ? row & 7 : w_key<KIND, TN>(row))) << 4;
-        const int64_t off = is_h ? min(row, t.row1 - 1 - t.row0) * (a.ldh * ES) : min(row, a.ctot - 1 - n0) * kbytes;
-        if constexpr (DIRECT) at0[i] = (int)off + koff[i];
-        else src[i] = (is_h ? Ht : Wt) + off;
+        const int last = is_h ? t.row1 - 1 - t.row0 : a.ctot - 1 - n0;
+        const int64_t stride = is_h ? a.ldh * ES : kbytes;
+        if constexpr (DIRECT) at0[i] = min(row, last) * (int)stride + koff[i];
+        else src[i] = (is_h ? Ht : Wt) + min(row, last) * stride;
     }
     constexpr bool W_PART = NW * T != BN * 8;  // the last W chunk belongs to the first waves only
     i32x4 reg[DIRECT ? 1 : NH + NW];
@@ -521,7 +524,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int64_t slots
 }
 
 template <int KIND, int BM, int BN, int WM, int WN, int NBUF, bool DIRECT>
-__global__ __launch_bounds__(WM* WN * 64) void k_product(ProductArgs a, int64_t slots, int col_tiles) {
+__global__ __launch_bounds__(WM* WN * 64) void k_product(ProductArgs a, int slots, int col_tiles) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     product_tile<KIND, BM, BN, WM, WN, NBUF, DIRECT>(a, slots, col_tiles, smem);
 }
@@ -530,13 +533,13 @@ __global__ __launch_bounds__(WM* WN * 64) void k_product(ProductArgs a, int64_t 
 // interleaved pieces of 128 bytes, read their fragments straight from memory (every weight is used once: LDS would only be a
 // detour) and join their sums through LDS in a fixed order.
 template <int KIND, int NT, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void k_product_few(ProductArgs a, int64_t slots, int col_tiles) {
+__global__ __launch_bounds__(WAVES * 64) void k_product_few(ProductArgs a, int slots, int col_tiles) {
     constexpr int ES = Elem<KIND>::size, BM = 16, BN = 16 * NT;
     using Acc = typename Elem<KIND>::Acc;
     __shared__ __attribute__((aligned(16))) Acc part[WAVES][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4;
     const int64_t kbytes = (int64_t)a.cin * ES;
-    const Tile t = find_tile<BM>(a, blockIdx.x, slots, col_tiles);
+    const Tile t = find_tile<BM>(a, (int)blockIdx.x, slots, col_tiles);
     if (t.row0 >= t.row1) return;
     const int n0 = t.col * BN;
     const char* h = a.H + (t.row0 + (int64_t)min(lane & 15, t.row1 - 1 - t.row0)) * a.ldh * ES;
@@ -546,8 +549,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_product_few(ProductArgs a, int64
         w[j] = a.W + ((int64_t)t.model * a.ctot + n0 + min(j * 16 + (lane & 15), a.ctot - 1 - n0)) * kbytes;
     Acc acc[NT] = {};
     const int pieces = (int)((kbytes + 127) >> 7);
-    // whole pieces; of rows that start anywhere, those that are neither first nor last
-    const int from = a.dwords ? 0 : 1, to = (int)((a.dwords ? kbytes : kbytes - 4) >> 7);
+    // whole pieces; where rows of W start anywhere, those that are neither first nor last
+    const int from = a.dwords_w ? 0 : 1, to = (int)((a.dwords_w ? kbytes : kbytes - 4) >> 7);
     constexpr int U = NT >= 4 ? 2 : 4;
     int c = wave;
     auto checked = [&](int c) {
@@ -559,8 +562,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_product_few(ProductArgs a, int64
             for (int j = 0; j < NT; ++j) acc[j] = mfma_step<KIND>(load_chunk(w[j], off, kbytes), fh, acc[j]);
         }
     };
-    auto whole = [&](auto dwords, int c, auto count) {
-        constexpr bool DW = decltype(dwords)::value;
+    auto whole = [&](auto dwords_w, int c, auto count) {
+        constexpr bool DW = decltype(dwords_w)::value;
         constexpr int N = decltype(count)::value;
         i32x4 fh[N][2], fw[N][2][NT];
 #pragma unroll
@@ -587,11 +590,11 @@ __global__ __launch_bounds__(WAVES * 64) void k_product_few(ProductArgs a, int64
         checked(c);
         c += WAVES;
     }
-    auto middle = [&](auto dwords) {
-        for (; c + (U - 1) * WAVES < to; c += U * WAVES) whole(dwords, c, std::integral_constant<int, U>{});
-        for (; c < to; c += WAVES) whole(dwords, c, std::integral_constant<int, 1>{});
+    auto middle = [&](auto dwords_w) {
+        for (; c + (U - 1) * WAVES < to; c += U * WAVES) whole(dwords_w, c, std::integral_constant<int, U>{});
+        for (; c < to; c += WAVES) whole(dwords_w, c, std::integral_constant<int, 1>{});
     };
-    if (ES == 4 || a.dwords) middle(std::true_type{});
+    if (a.dwords_w) middle(std::true_type{});
     else middle(std::false_type{});
     if (c < pieces) checked(c);  // (one of at most two last pieces)
 #pragma unroll
@@ -760,11 +763,19 @@ static int launch_tiles_as(const char* family, const ProductArgs& a, hipStream_t
     const int col_tiles = (a.ctot + BN - 1) / BN;
     if (slots * col_tiles > max_grid(WM * WN * 64)) return fail(DGCN_ERR_UNSUPPORTED, "%s: %lld tiles in one call", family, (long long)(slots * col_tiles));
     const int lds = (int)min(((int64_t)a.cin * Elem<KIND>::size - 1) / kRowBytes + 1, (int64_t)NBUF) * (BM + BN) * kRowBytes;
-    if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product<KIND, BM, BN, WM, WN, NBUF, DIRECT>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, NBUF * (BM + BN) * kRowBytes) != hipSuccess)
-        return fail(DGCN_ERR_LAUNCH, "%s: %d bytes of LDS are not available", family, lds);
+    if (lds > 64 * 1024) {
+        static std::atomic<int> reserved[64];
+        int dev = 0;
+        (void)hipGetDevice(&dev);
+        if (!reserved[dev & 63].load(std::memory_order_relaxed)) {
+            if (hipFuncSetAttribute(reinterpret_cast<const void*>(&k_product<KIND, BM, BN, WM, WN, NBUF, DIRECT>),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, NBUF * (BM + BN) * kRowBytes) != hipSuccess)
+                return fail(DGCN_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS", family, lds);
+            reserved[dev & 63].store(1, std::memory_order_relaxed);
+        }
+    }
     TimedLaunch t(family, s);
-    DGCN_LAUNCH(t, (k_product<KIND, BM, BN, WM, WN, NBUF, DIRECT>), dim3((unsigned)(slots * col_tiles)), dim3(WM * WN * 64), lds, s, a, slots, col_tiles);
+    DGCN_LAUNCH(t, (k_product<KIND, BM, BN, WM, WN, NBUF, DIRECT>), dim3((unsigned)(slots * col_tiles)), dim3(WM * WN * 64), lds, s, a, (int)slots, col_tiles);
     return check_launch("k_product");
 }
 
@@ -786,7 +797,7 @@ template <int KIND, int NT, int WAVES> static int launch_few(const char* family,
     const int col_tiles = (a.ctot + 16 * NT - 1) / (16 * NT);
     if (slots * col_tiles > max_grid(WAVES * 64)) return fail(DGCN_ERR_UNSUPPORTED, "%s: %lld tiles in one call", family, (long long)(slots * col_tiles));
     TimedLaunch t(family, s);
-    DGCN_LAUNCH(t, (k_product_few<KIND, NT, WAVES>), dim3((unsigned)(slots * col_tiles)), dim3(WAVES * 64), 0, s, a, slots, col_tiles);
+    DGCN_LAUNCH(t, (k_product_few<KIND, NT, WAVES>), dim3((unsigned)(slots * col_tiles)), dim3(WAVES * 64), 0, s, a, (int)slots, col_tiles);
     return check_launch("k_product_few");
 }
 
@@ -814,6 +825,7 @@ template <int KIND, int TN, int KS> static int launch_rows(const char* family, c
 // 26 (the others: many groups of few rows, up to 35 %).
 struct Shape { int bm, bn, per_cu; float s1, sc, f; };
 constexpr int kShapes = 5;
+constexpr float kBytesPerUs = 4.7e6f;  // a large copy, read and written
 constexpr Shape kDirect[kShapes] = {{64, 64, 5, .55f, 1.11f, 2.f}, {128, 128, 2, .78f, 1.05f, 3.f}, {128, 256, 1, .98f, .98f, 4.f},
                                     {192, 256, 1, 1.36f, 1.36f, 5.f}, {256, 256, 1, 1.8f, 1.8f, 6.f}};
 constexpr Shape kStaged[kShapes] = {{64, 64, 4, .85f, 1.6f, 2.f}, {128, 128, 1, 1.23f, 1.23f, 3.f}, {128, 256, 1, 1.7f, 1.7f, 4.f},
@@ -821,7 +833,7 @@ constexpr Shape kStaged[kShapes] = {{64, 64, 4, .85f, 1.6f, 2.f}, {128, 128, 1, 
 
 // Row tiles a launch is expected to have: the host knows rows and groups, not the groups' sizes.
 static float expected_slots(const ProductArgs& a, int BM) {
-    if (!a.gptr) return (float)(((int64_t)a.rows + BM - 1) / BM);
+    if (!a.gptr || a.num_groups == 1) return (float)(((int64_t)a.rows + BM - 1) / BM);
     return (float)a.rows / BM + .5f * min(a.num_groups, a.rows);
 }
 
@@ -839,10 +851,12 @@ static int choose_shape(const ProductArgs& a, int64_t row_bytes, bool direct) {
         if (rest > .02f) cost += (p.s1 + (p.per_cu > 1 ? (p.sc - p.s1) * (ceilf(rest) - 1.f) / (p.per_cu - 1) : 0.f)) * steps + p.f;
         if (cost < least) { least = cost; best = i; }
     }
-    // Groups of so few rows that the weights are nearly all the bytes, and those bytes are the time: 128 x 128 reads them once more seldom
-    // (64 groups, 2 048 rows, 2 048 bytes x 1 024 columns: 27.8 us against 37.5 of the 64 x 64 tile).
-    const float weights = (float)min(a.num_groups, a.rows) * a.ctot * row_bytes, rest = (float)a.rows * (row_bytes + 2.f * a.ctot);
-    if (direct && a.gptr && weights > 4.f * rest && weights / 4.7e6f > least) best = 1;
+    // Where the bytes alone take longer than that, a copy's many small workgroups are best (100 000 rows, int8 128 -> 256 float32: 26 us
+    // with 64 x 64 and 128 x 128, 30 .. 35 with the larger ones) - unless nearly all of them are weights of groups with few rows,
+    // which 128 x 128 reads more seldom (64 groups, 2 048 rows, 2 048 bytes x 1 024 columns: 28 us against 37 of 64 x 64).
+    const float weights = (float)(a.gptr ? min(a.num_groups, a.rows) : 1) * a.ctot * row_bytes;
+    const float others = (float)a.rows * (row_bytes + (a.out_dtype == DGCN_F32 ? 4.f : 2.f) * a.ctot);
+    if ((weights + others) / kBytesPerUs > least) best = a.gptr && weights > 4.f * others ? 1 : 0;
     return best;
 }
 
@@ -853,7 +867,7 @@ template <int KIND> static int dispatch_kind(const char* family, const ProductAr
     } else {
         // a narrow layer over very many rows: no tile would be more than a copy (800 000 rows of 32 float32 -> 2: 28 us against 32 of the
         // 128 x 16 tile; 300 000 rows of 32 bf16 -> 32: 12 against 19 of 64 x 64; at 60 000 rows no difference)
-        if (a.H && a.dwords && row_bytes % 16 == 0 && row_bytes <= 128 && a.ctot <= 32 && a.rows >= 1 << 17)
+        if (a.H && a.dwords_h && a.dwords_w && row_bytes % 16 == 0 && row_bytes <= 128 && a.ctot <= 32 && a.rows >= 1 << 17)
             return a.ctot <= 16 ? launch_rows<KIND, 1, 2>(family, a, s) : launch_rows<KIND, 2, 2>(family, a, s);
     }
     const int groups = min(a.num_groups, a.rows);
@@ -888,7 +902,8 @@ template <int KIND> static int dispatch_kind(const char* family, const ProductAr
 
 static int product_dispatch(const char* family, int kind, ProductArgs& a, hipStream_t s) {
     const int es = kind == K_I8 ? 1 : kind == K_BF16 || kind == K_F16 ? 2 : 4;
-    a.dwords = es == 4 || (((uintptr_t)a.H | (uintptr_t)a.W) % 4 == 0 && a.ldh * es % 4 == 0 && (int64_t)a.cin * es % 4 == 0);
+    a.dwords_h = (uintptr_t)a.H % 4 == 0 && a.ldh * es % 4 == 0;
+    a.dwords_w = (uintptr_t)a.W % 4 == 0 && (int64_t)a.cin * es % 4 == 0;
     switch (kind) {
         case K_I8: return dispatch_kind<K_I8>(family, a, s);
         case K_BF16: return dispatch_kind<K_BF16>(family, a, s);

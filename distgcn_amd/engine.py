@@ -103,13 +103,14 @@ def _matrix(x, what, dtypes, cols=None, rows=None):
     if len(shape) != 2 or (cols is not None and shape[1] != cols) or (rows is not None and shape[0] != rows):
         raise ValueError("%s has shape %s, expected [%s, %s]" % (what, tuple(shape), "rows" if rows is None else rows,
                                                                  "columns" if cols is None else cols))
+    r, c = shape
     ld, inner = x.stride()
-    if shape[1] > 1 and inner != 1:
+    if inner != 1 and c > 1:
         raise ValueError("%s: the entries of a row must be contiguous" % what)
-    if shape[0] <= 1:
-        return max(int(shape[1]), 1)
-    if ld < shape[1]:
-        raise ValueError("%s: rows overlap (row stride %d, %d columns)" % (what, ld, shape[1]))
+    if r <= 1:
+        return max(c, 1)
+    if ld < c:
+        raise ValueError("%s: rows overlap (row stride %d, %d columns)" % (what, ld, c))
     return ld
 
 
@@ -117,7 +118,7 @@ def _array(x, what, dtype, shape):
     """Check a contiguous tensor of one dtype and shape."""
     if x.dtype != dtype:
         raise TypeError("%s is %s, expected %s" % (what, x.dtype, dtype))
-    if tuple(x.shape) != shape:
+    if x.shape != shape:
         raise ValueError("%s has shape %s, expected %s" % (what, tuple(x.shape), shape))
     if not x.is_contiguous():
         raise ValueError("%s must be contiguous" % what)
@@ -133,6 +134,9 @@ class Engine:
         self.lib = _lib.load()
         self._table = None
         self._ws = None
+        self._codes = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}  # the products' floating-point types
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (the same handle without building a Stream object)
+        self._raw_stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
     # ------------------------------------------------------------------ helpers
     def _stream(self):
@@ -279,32 +283,32 @@ class Engine:
         return out
 
     # ------------------------------------------------------------------ K2/K3 for several models / in 8-bit integers
-    def _codes(self):
-        """{torch dtype: DGCN_* code} of the products' floating-point types."""
-        t = self.torch
-        return {t.float32: _lib.F32, t.bfloat16: _lib.BF16, t.float16: _lib.F16}
+    def _index(self):
+        """Number of this engine's device."""
+        index = self.device.index
+        return self.torch.cuda.current_device() if index is None else index
 
     def _here(self, *tensors):
         """Every tensor (None: not given) lives on this engine's device."""
-        index = self.device.index
-        if index is None:
-            index = self.torch.cuda.current_device()
+        index = self._index()
         for x in tensors:
-            if x is not None and (x.device.type != self.device.type or x.device.index != index):
+            if x is not None and x.get_device() != index:
                 raise ValueError("a tensor is on %s, the engine on %s" % (x.device, self.device))
 
     def _launch(self, fn, what, *args):
-        """One library call on this engine's device and current stream."""
-        index = self.device.index
-        if index is None or index == self.torch.cuda.current_device():
-            _lib.check(fn(*args, self._stream()), what)
+        """One library call on this engine's device and its current stream."""
+        index = self._index()
+        if index == self.torch.cuda.current_device():
+            rc = fn(*args, self._raw_stream(index))
         else:
             with self.torch.cuda.device(index):
-                _lib.check(fn(*args, self._stream()), what)
+                rc = fn(*args, self._raw_stream(index))
+        if rc:
+            _lib.check(rc, what)
 
     def _product_args(self, H, W, bias, act, dtype, out, grouped, rows=None):
         """The checks every product shares -> (rows, cin, ctot, models, ldh, activation code, dtype code, out, ldy)."""
-        codes = self._codes()
+        codes = self._codes
         if dtype not in codes:
             raise TypeError("dtype is %s, expected %s" % (dtype, " / ".join(str(d) for d in codes)))
         if act not in ACT_CODES:
@@ -353,8 +357,8 @@ class Engine:
         quantises weights, a row per output column.  ``out = (q, scale)`` re-uses buffers.  -> (int8 [rows, cols], float32 [rows]);
         a row with a NaN or an infinity gets scale NaN."""
         t = self.torch
-        codes = self._codes()
-        ldx = _matrix(X, "X", tuple(codes))
+        codes = self._codes
+        ldx = _matrix(X, "X", codes)
         rows, cols = X.shape
         if out is None:
             q, scale = t.empty((rows, cols), dtype=t.int8, device=self.device), t.empty(rows, dtype=t.float32, device=self.device)
