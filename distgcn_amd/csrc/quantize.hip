@@ -127,16 +127,20 @@ static int launch_quantize_as(const void* X, int64_t ldx, int rows, int cols, in
 
 template <class T> static int launch_quantize(const void* X, int64_t ldx, int rows, int cols, int8_t* Q, int64_t ldq, float* scale, hipStream_t s) {
 #define DGCN_Q_CASE(LPR, UN, LOOP) return launch_quantize_as<T, LPR, UN, LOOP>(X, ldx, rows, cols, Q, ldq, scale, s)
+    // The fewest lanes that hold a row in four units each: several rows' loads are in flight per wave and less of it idles behind a
+    // row's end (100 000 rows of 500 float32: 51 us, a wave per row with one unit 61; 333 bf16: 32 against 54; 16 384 rows of 1 000 fp16: 12
+    // against 25 with a workgroup per row, 2 048 bf16: 26 against 35).  From 2 049 columns on a workgroup per row: 4 096 bf16 47 us, a
+    // wave with eight units 64.
     const int units = (cols - 1) / kUnit + 1;
     if (units <= 1) DGCN_Q_CASE(1, 1, false);
     if (units <= 2) DGCN_Q_CASE(2, 1, false);
     if (units <= 4) DGCN_Q_CASE(4, 1, false);
-    if (units <= 8) DGCN_Q_CASE(8, 1, false);
-    if (units <= 16) DGCN_Q_CASE(16, 1, false);
-    if (units <= 32) DGCN_Q_CASE(32, 1, false);
-    if (units <= 64) DGCN_Q_CASE(64, 1, false);
-    // (a workgroup per row; units that a lane holds at once keep loads in flight: 4 096 bf16 columns 46 us with two, 75 with 512 lanes and one)
-    if (units <= 256) DGCN_Q_CASE(256, 1, false);
+    if (units <= 8) DGCN_Q_CASE(4, 2, false);
+    if (units <= 16) DGCN_Q_CASE(4, 4, false);
+    if (units <= 32) DGCN_Q_CASE(8, 4, false);
+    if (units <= 64) DGCN_Q_CASE(16, 4, false);
+    if (units <= 128) DGCN_Q_CASE(64, 2, false);
+    if (units <= 256) DGCN_Q_CASE(64, 4, false);
     if (units <= 512) DGCN_Q_CASE(256, 2, false);
     if (units <= 1024) DGCN_Q_CASE(256, 4, false);
     DGCN_Q_CASE(1024, 4, true);

@@ -469,6 +469,8 @@ class Engine:
         objects with such ``.layers``, e.g. ``gcn.models.GCN_DQN``).  ``precision="int8"``: the products of the hidden layers run in 8-bit integers
         with scales per vertex and output column; the first and the last layer stay in float32 (as do all aggregations)."""
         t = self.torch
+        if any(getattr(m, "has_head", False) for m in models):
+            raise _lib.DgcnError("a bank takes models whose output is their last layer (no is_dual / skip head)")
         models = [getattr(m, "layers", m) for m in models]
         if not models or not models[0]:
             raise ValueError("a bank needs at least one model with at least one layer")

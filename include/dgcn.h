@@ -236,12 +236,15 @@ int dgcn_transform_f64acc_batch(const float* H, int32_t ldh, float h_const, int3
  *    before the first and behind the last group are left as they were.  DGCN_FAULT_BAD_GROUP in *status (required; the caller
  *    zeroes it once): a pointer that decreases or leaves [0, rows], a model id outside [0, num_models) - that group's rows are
  *    left as they were (bad pointers: clamped, contents of Y's rows then undefined).
- *  - act is applied behind the bias.  No atomics but the status word, no workspace: a row's result depends on that row, its model
- *    and the call's sizes (rows, num_groups, cin, ctot, types) only, and repeated calls return the same bits.
+ *  - act is applied behind the bias.  Y / Q must not overlap the inputs.  No atomics but the status word, no workspace, nothing kept
+ *    between calls: a row's result depends on that row, its model and the call's sizes, types and alignment only (float32: on the row
+ *    and its model), and repeated calls return the same bits.
+ *  - Any alignment the element type has is taken; rows of H and W at multiples of 16 bytes are fastest (bytes at odd addresses: about half
+ *    the rate).  DGCN_ERR_UNSUPPORTED: more than 2^31 - 1 024 rows or columns, or a call of more than some 2^24 tiles of 64 x 64.
  *
  * dgcn_quantize_rows_batch: Q[r][k] = x / scale[r] rounded half to even (exact quotient), |Q| <= 127;
  *   scale[r] = max(max_k |X[r][k]| / 127, 2^-126) in float32.  A row with a NaN or an infinity gets scale NaN and Q = 0, so that every
- *   product of that row is NaN.  X: float32 / bf16 / fp16 (dtype).  Q must not overlap X.
+ *   product of that row is NaN.  X: float32 / bf16 / fp16 (dtype).
  * dgcn_transform_int8_batch: Y[r][n] = act(((float)acc * h_scale[r]) * w_scale[n] + bias[n]), acc = sum_k H[r][k] W[n][k] exact in
  *   int32 (cin <= 131071), float32 arithmetic behind it, rounded once to out_dtype.
  * dgcn_transform_grouped_batch: Y[r][n] = act(sum_k H[r][k] W[e][n][k] + bias[e][n]), e the model of r's group; H, W and Y are of

@@ -269,6 +269,20 @@ def test_grouped_constant_features(engine):
     for g, (lo, hi) in enumerate(blocks):
         if hi > lo:
             assert torch.equal(y[lo:hi], engine.transform(None, W[g].t().contiguous(), rows=hi - lo, h_const=float(np.float32(1 / 19))))
+    p = engine.transform_grouped(None, W, ptr, rows=93, h_const=0.3, precise=True)
+    assert torch.equal(p[:10], engine.transform(None, W[0].t().contiguous(), rows=10, h_const=0.3, precise=True))
+
+
+@pytest.mark.parametrize("rows,cin,ctot", [(3, 64, 20), (70, 64, 70), (5, 512, 64), (300, 700, 130), (140000, 64, 16)])
+def test_subnormal_inputs_count(engine, rows, cin, ctot):
+    """fp16 values below 2^-14 and bf16 / float32 values below 2^-126 enter the products as they are (the sums here are exact)."""
+    import torch
+    ptr, _ = _groups([rows])
+    for dtype, tiny in ((torch.float16, 2.0 ** -24), (torch.bfloat16, 2.0 ** -133), (torch.float32, 2.0 ** -149)):
+        H = torch.full((rows, cin), tiny, dtype=dtype, device="cuda:0")
+        W = torch.full((1, ctot, cin), 2.0, dtype=dtype, device="cuda:0")
+        y = engine.transform_grouped(H, W, ptr)
+        assert bool((y.double() == 2 * cin * tiny).all()), dtype
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])

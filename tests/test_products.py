@@ -144,6 +144,11 @@ def test_bank_refusals(host_engine):
     for models, kw in (([], {}), ([[]], {}), ([a, datagen.random_model(4, 8)], {}), ([a, datagen.random_model(3, 16)], {}), ([a], dict(precision="int4"))):
         with pytest.raises(ValueError):
             e.model_bank(models, **kw)
+    from distgcn_amd.gcn.models import GCN2_DQN, GCN_DQN
+    nets = [GCN2_DQN(hidden_dim=8, num_layer=3, input_dim=1, max_degree=1, wts_init="random", seed=s) for s in (1, 2)]
+    assert e.model_bank(nets).layers[2]["act"] == "leaky_relu" and e.model_bank(nets, precision="float32").num_models == 2
+    with pytest.raises(_lib.DgcnError, match="head"):
+        e.model_bank([GCN2_DQN(hidden_dim=8, num_layer=2, input_dim=1, max_degree=1, wts_init="random", output_dim=3, is_dual=True)])
     with pytest.raises(_lib.DgcnError, match="supports"):
         e.model_bank([[dict(lyr, weights=lyr["weights"] + [lyr["weights"][0]]) for lyr in a]])
 
