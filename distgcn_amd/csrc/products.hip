@@ -492,12 +492,16 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int slots, in
                     multiply_rows(p, 0, AHEAD ? 1 : RT);
                 }
                 if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
+                if (!DIRECT && p == PHASES - 2 && st + 1 < steps) {
+                    // (everyone left the buffer of stage st - 1 at the last barrier; a phase is left to hide these writes behind)
+                    deposit(next);
+                    if (st + 2 < steps) fetch(st + 2, cur);
+                }
                 if (last && st + 1 < steps) {
                     // stage st + 1 lies in its buffer, everyone has read all of stage st
-                    deposit(next);
                     if (NBUF == 3 && st + 2 < steps) arrive_all<DIRECT, NH + NW>();
                     else arrive_all<DIRECT, 0>();
-                    if (st + NBUF < steps) fetch(st + NBUF, cur);
+                    if (DIRECT && st + NBUF < steps) fetch(st + NBUF, cur);
                 }
                 if constexpr (AHEAD) {
                     if (!last ? ALL || (p + 1) % HALVES < live : st + 1 < steps && (ALL || live > 0))
