@@ -35,6 +35,7 @@ struct ProductArgs {
     float h_const;
     int rows, cin, ctot, num_groups, num_models, act, out_dtype;
     bool dwords_h, dwords_w;  // rows of H, of W start at multiples of 4 bytes
+    bool stream;              // Y is stored past the caches (see streams_out)
 };
 
 template <int KIND> struct Elem;
@@ -224,7 +225,14 @@ __device__ __forceinline__ void finish(const ProductArgs& a, int64_t r, int n, c
     for (int i = 0; i < CH; ++i) o[i] = (O)x[i];
     O* y = reinterpret_cast<O*>(a.Y) + r * a.ldy + n;
     if (n + CH <= a.ctot) {
-        __builtin_memcpy(y, &o, sizeof(o));
+        if (sizeof(o) % 16 == 0 && a.stream) {
+            i32x4 piece[sizeof(o) / 16 + (sizeof(o) < 16)];
+            __builtin_memcpy(piece, &o, sizeof(o));
+#pragma unroll
+            for (int i = 0; i < (int)(sizeof(o) / 16); ++i) __builtin_nontemporal_store(piece[i], reinterpret_cast<i32x4*>(y) + i);
+        } else {
+            __builtin_memcpy(y, &o, sizeof(o));
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < CH - 1; ++i)
@@ -841,7 +849,20 @@ static float expected_slots(const ProductArgs& a, int BM) {
     return (float)a.rows / BM + .5f * min(a.num_groups, a.rows);
 }
 
-static int choose_shape(const ProductArgs& a, int64_t row_bytes, bool direct) {
+// Bytes of a call: every model's weights once, every row in and out.
+static float weight_bytes(const ProductArgs& a, int64_t row_bytes) { return (float)(a.gptr ? min(a.num_groups, a.rows) : 1) * a.ctot * row_bytes; }
+static float out_bytes(const ProductArgs& a) { return (float)a.rows * (a.out_dtype == DGCN_F32 ? 4.f : 2.f) * a.ctot; }
+
+// A call that takes about as long as its bytes do (`compute_us`: without them) and whose bytes are mostly Y stores it past the caches, in whole
+// 16-byte pieces: 100 000 rows, int8 128 -> 256 float32 41 -> 26 us with outputs that the caches do not already hold; the six layers
+// of a 128-wide 8-bit bank over 500 graphs 615 -> 576 us, aggregations included.  Calls that compute for longer lose by it (fp32 128 -> 256: 1 %).
+static bool streams_out(const ProductArgs& a, int64_t row_bytes, float compute_us) {
+    const int os = a.out_dtype == DGCN_F32 ? 4 : 2;
+    const float out = out_bytes(a), all = out + weight_bytes(a, row_bytes) + (float)a.rows * row_bytes;
+    return all / kBytesPerUs > .75f * compute_us && out > .5f * all && a.ldy * os % 16 == 0 && (uintptr_t)a.Y % 16 == 0;
+}
+
+static int choose_shape(ProductArgs& a, int64_t row_bytes, bool direct) {
     const Shape* shapes = direct ? kDirect : kStaged;
     const float steps = (float)((row_bytes + kRowBytes - 1) / kRowBytes);
     int best = 0;
@@ -855,16 +876,17 @@ static int choose_shape(const ProductArgs& a, int64_t row_bytes, bool direct) {
         if (rest > .02f) cost += (p.s1 + (p.per_cu > 1 ? (p.sc - p.s1) * (ceilf(rest) - 1.f) / (p.per_cu - 1) : 0.f)) * steps + p.f;
         if (cost < least) { least = cost; best = i; }
     }
-    // Where the bytes alone take longer than that, a copy's many small workgroups are best (100 000 rows, int8 128 -> 256 float32: 26 us
-    // with 64 x 64 and 128 x 128, 30 .. 35 with the larger ones) - unless nearly all of them are weights of groups with few rows,
-    // which 128 x 128 reads more seldom (64 groups, 2 048 rows, 2 048 bytes x 1 024 columns: 28 us against 37 of 64 x 64).
-    const float weights = (float)(a.gptr ? min(a.num_groups, a.rows) : 1) * a.ctot * row_bytes;
-    const float others = (float)a.rows * (row_bytes + (a.out_dtype == DGCN_F32 ? 4.f : 2.f) * a.ctot);
-    if ((weights + others) / kBytesPerUs > least) best = a.gptr && weights > 4.f * others ? 1 : 0;
+    // Where the bytes alone take longer than that, a copy's many small workgroups are best (100 000 rows, int8 127 -> 256: 33 us with 64 x 64,
+    // 41 .. 50 with the larger ones) - unless Y is stored past the caches, where whole 128-byte lines count, or nearly all of the bytes
+    // are weights of groups with few rows, which 128 x 128 reads more seldom (64 groups, 2 048 rows, 2 048 bytes x 1 024 columns: 28 us
+    // against 37 of 64 x 64).
+    a.stream = streams_out(a, row_bytes, least);
+    const float weights = weight_bytes(a, row_bytes), others = (float)a.rows * row_bytes + out_bytes(a);
+    if (a.stream || (weights + others) / kBytesPerUs > least) best = direct && (a.stream || (a.gptr && weights > 4.f * others)) ? 1 : 0;
     return best;
 }
 
-template <int KIND> static int dispatch_kind(const char* family, const ProductArgs& a, hipStream_t s) {
+template <int KIND> static int dispatch_kind(const char* family, ProductArgs& a, hipStream_t s) {
     const int64_t row_bytes = (int64_t)a.cin * Elem<KIND>::size;
     if constexpr (KIND == K_F32P) {
         return launch_tiles<KIND, 64, 64, 2, 2, 2>(family, a, s);
@@ -875,6 +897,7 @@ template <int KIND> static int dispatch_kind(const char* family, const ProductAr
             return a.ctot <= 16 ? launch_rows<KIND, 1, 2>(family, a, s) : launch_rows<KIND, 2, 2>(family, a, s);
     }
     const int groups = min(a.num_groups, a.rows);
+    if constexpr (KIND == K_F32) a.stream = streams_out(a, row_bytes, (float)a.rows * a.ctot * a.cin * 2.f / 149e6f);
     if constexpr (KIND == K_F32) {
         // float32: the matrix pipe is the bound from some 64 columns on, so the shape matters little but for its waste.  128 x 128 (1 024
         // x 1 024, 8 192 rows: 144 us against 165) where its tiles fill whole rounds of two per CU; 64 x 64 where a row is one stage (32
