@@ -256,45 +256,49 @@ __device__ __forceinline__ void column_values(const ProductArgs& a, int model, i
     }
 }
 
-// One wave's TM x TN tiles.  Columns come in pairs of tiles where TN is even (see w_row): a lane holds 8 neighbouring columns.
+// 16-bit results come in pairs of tiles where TN is even: a lane's columns of two tiles are neighbours and leave in one 16-byte store.
+template <int TN, class O> constexpr bool kPairs = sizeof(O) == 2 && TN % 2 == 0;
+template <int KIND, int TN> __device__ __forceinline__ bool in_pairs(const ProductArgs& a) {
+    if constexpr (TN % 2 != 0 || KIND == K_F32 || KIND == K_F32P) return false;
+    else if constexpr (KIND == K_I8) return a.out_dtype != DGCN_F32;
+    else return true;
+}
+// The output column (within a wave's columns) that MFMA row i of tile j computes.  An MFMA leaves rows 4 q .. 4 q + 3 in lane group q
+// (double: rows q, q + 4, ..): columns are dealt so that a lane group's 4 - in pairs of tiles 8 - are neighbours.
+template <int KIND> __device__ __forceinline__ int w_row(int i, int j, bool pairs) {
+    if constexpr (KIND == K_F32P) return j * 16 + 4 * (i & 3) + (i >> 2);
+    else return pairs ? (j >> 1) * 32 + (i >> 2) * 8 + (j & 1) * 4 + (i & 3) : j * 16 + i;
+}
+// The chunk permutation of an LDS row of W: eight lanes in a row read eight different bank groups.
+__device__ __forceinline__ int w_key(int row, bool pairs) { return pairs ? (row & 3) | ((row >> 1) & 4) : row & 7; }
+
+// One wave's TM x TN tiles.
 template <int KIND, class O, int TM, int TN>
 __device__ __forceinline__ void write_tiles(const ProductArgs& a, const Tile& t, int row, int col, const typename Elem<KIND>::Acc (&acc)[TM][TN]) {
-    constexpr int PW = TN % 2 == 0 && KIND != K_F32P ? 2 : 1, CH = 4 * PW;
+    constexpr int PW = kPairs<TN, O> ? 2 : 1, CH = 4 * PW;
     const int lane = threadIdx.x & 63, q = lane >> 4;
     float hs[TM];
     if constexpr (KIND == K_I8) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) hs[i] = a.hs[t.row0 + (int64_t)min(row + i * 16 + (lane & 15), t.row1 - 1 - t.row0)];
     }
+    float ws[TN / PW][CH], bias[TN / PW][CH];
 #pragma unroll
-    for (int p = 0; p < TN / PW; ++p) {
-        const int n = col + p * 16 * PW + q * CH;
-        if (n >= a.ctot) continue;
-        float ws[CH], bias[CH];
-        column_values<KIND, CH>(a, t.model, n, ws, bias);
+    for (int p = 0; p < TN / PW; ++p) column_values<KIND, CH>(a, t.model, min(col + p * 16 * PW + q * CH, a.ctot - 1), ws[p], bias[p]);
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int64_t r = (int64_t)t.row0 + row + i * 16 + (lane & 15);
-            if (r >= t.row1) continue;
+    for (int i = 0; i < TM; ++i) {
+        const int64_t r = (int64_t)t.row0 + row + i * 16 + (lane & 15);
+        if (r >= t.row1) continue;
+#pragma unroll
+        for (int p = 0; p < TN / PW; ++p) {  // (a row's columns one behind the other: its lines leave the caches whole)
+            const int n = col + p * 16 * PW + q * CH;
+            if (n >= a.ctot) continue;
             float v[CH];
 #pragma unroll
             for (int x = 0; x < CH; ++x) v[x] = (float)acc[i][p * PW + (x >> 2)][x & 3];
-            finish<KIND, O, CH>(a, r, n, v, KIND == K_I8 ? hs[i] : 0.f, ws, bias);
+            finish<KIND, O, CH>(a, r, n, v, KIND == K_I8 ? hs[i] : 0.f, ws[p], bias[p]);
         }
     }
-}
-
-// The output column (within a wave's columns) that MFMA row i of tile j computes.  An MFMA leaves rows 4 q .. 4 q + 3 in lane group q
-// (double: rows q, q + 4, ..): tiles in pairs deal their columns so that a lane group's 8 (alone: 4) are neighbours.
-template <int KIND, int TN> __device__ __forceinline__ int w_row(int i, int j) {
-    if constexpr (KIND == K_F32P) return j * 16 + 4 * (i & 3) + (i >> 2);
-    else if constexpr (TN % 2 == 0) return (j >> 1) * 32 + (i >> 2) * 8 + (j & 1) * 4 + (i & 3);
-    else return j * 16 + i;
-}
-// The chunk permutation of an LDS row of W: eight lanes in a row read eight different bank groups.
-template <int KIND, int TN> __device__ __forceinline__ int w_key(int row) {
-    if constexpr (TN % 2 == 0 && KIND != K_F32P) return (row & 3) | ((row >> 1) & 4);
-    else return row & 7;
 }
 
 // 16 bytes at byte offset `off` of a row of `row_bytes` bytes, any alignment; bytes behind the row's end are zero: a chunk that crosses
@@ -373,6 +377,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int slots, in
     const int n0 = t.col * BN;
     const char* Wm = a.W + (int64_t)t.model * a.ctot * kbytes;
 
+    const bool pairs = in_pairs<KIND, TN>(a);
     // this thread's chunks: number c of the buffer lies at byte 16 c, row c / 8, and holds chunk (c % 8) ^ (row's key) of that row
     const char* src[DIRECT ? 1 : NH + NW];
     int at0[DIRECT ? NH + NW : 1];  // DIRECT: byte offset from the tile's first row
@@ -383,7 +388,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int slots, in
     for (int i = 0; i < NH + NW; ++i) {
         const bool is_h = i < NH;
         const int c = (is_h ? i : i - NH) * T + tid, row = c >> 3;
-        koff[i] = ((c & 7) ^ (is_h ? row & 7 : w_key<KIND, TN>(row))) << 4;
+        koff[i] = ((c & 7) ^ (is_h ? row & 7 : w_key(row, pairs))) << 4;
         const int last = is_h ? t.row1 - 1 - t.row0 : a.ctot - 1 - n0;
         const int64_t stride = is_h ? a.ldh * ES : kbytes;
         if constexpr (DIRECT) at0[i] = min(row, last) * (int)stride + koff[i];
@@ -453,8 +458,8 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int slots, in
         if (half == 0) {
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
-                const int row = w_row<KIND, TN>(lane & 15, j);
-                fw[AHEAD ? k : 0][j] = lds_frag<KIND, RB>(sW, wn + row, w_key<KIND, TN>(row), k);
+                const int row = w_row<KIND>(lane & 15, j, pairs);
+                fw[AHEAD ? k : 0][j] = lds_frag<KIND, RB>(sW, wn + row, w_key(row, pairs), k);
             }
         }
 #pragma unroll
@@ -719,14 +724,14 @@ __device__ __forceinline__ void product_rows(const ProductArgs& a, int run) {
                     model = e;
 #pragma unroll
                     for (int j = 0; j < TN; ++j) {
-                        const char* row = a.W + ((int64_t)e * a.ctot + min(w_row<KIND, TN>(lane & 15, j), a.ctot - 1)) * kbytes;
+                        const char* row = a.W + ((int64_t)e * a.ctot + min(w_row<KIND>(lane & 15, j, kPairs<TN, O>), a.ctot - 1)) * kbytes;
 #pragma unroll
                         for (int k = 0; k < KS; ++k) {
                             w[j][k] = i32x4{0, 0, 0, 0};
                             if (k * 64 + q * 16 < kbytes) __builtin_memcpy(&w[j][k], row + k * 64 + q * 16, 16);
                             w[j][k] = chain_order<KIND>(w[j][k]);
                         }
-                        column_values<KIND, 4>(a, e, min(w_row<KIND, TN>(4 * q, j), a.ctot - 1), ws[j], bias[j]);
+                        column_values<KIND, 4>(a, e, min(w_row<KIND>(4 * q, j, kPairs<TN, O>), a.ctot - 1), ws[j], bias[j]);
                     }
                 }
                 Acc acc[TN] = {};
@@ -737,7 +742,7 @@ __device__ __forceinline__ void product_rows(const ProductArgs& a, int run) {
                 const int64_t row = window + (lane & 15);
                 if (row >= r && row < stop) {
                     const float hs = KIND == K_I8 ? a.hs[row] : 0.f;
-                    constexpr int PW = TN % 2 == 0 ? 2 : 1, CH = 4 * PW;
+                    constexpr int PW = kPairs<TN, O> ? 2 : 1, CH = 4 * PW;
 #pragma unroll
                     for (int p = 0; p < TN / PW; ++p) {
                         const int n = p * 16 * PW + q * CH;
@@ -853,13 +858,14 @@ static float expected_slots(const ProductArgs& a, int BM) {
 static float weight_bytes(const ProductArgs& a, int64_t row_bytes) { return (float)(a.gptr ? min(a.num_groups, a.rows) : 1) * a.ctot * row_bytes; }
 static float out_bytes(const ProductArgs& a) { return (float)a.rows * (a.out_dtype == DGCN_F32 ? 4.f : 2.f) * a.ctot; }
 
-// A call that takes about as long as its bytes do (`compute_us`: without them) and whose bytes are mostly Y stores it past the caches, in whole
-// 16-byte pieces: 100 000 rows, int8 128 -> 256 float32 41 -> 26 us with outputs that the caches do not already hold; the six layers
-// of a 128-wide 8-bit bank over 500 graphs 615 -> 576 us, aggregations included.  Calls that compute for longer lose by it (fp32 128 -> 256: 1 %).
+// A call that takes about as long as its bytes do (`compute_us`: without them) and whose bytes are mostly Y stores it past the caches, in
+// whole 64-byte sectors (rows of 4 000 bytes, which are not, take twice as long that way): 100 000 rows, int8 128 -> 256 float32 24 us
+// against 40 with outputs that the caches do not already hold; the six layers of a 128-wide 8-bit bank over 500 graphs 565 us against
+// 615, aggregations included.  Calls that compute for longer lose by it (fp32 128 -> 256: 1 %).
 static bool streams_out(const ProductArgs& a, int64_t row_bytes, float compute_us) {
     const int os = a.out_dtype == DGCN_F32 ? 4 : 2;
     const float out = out_bytes(a), all = out + weight_bytes(a, row_bytes) + (float)a.rows * row_bytes;
-    return all / kBytesPerUs > .75f * compute_us && out > .5f * all && a.ldy * os % 16 == 0 && (uintptr_t)a.Y % 16 == 0;
+    return all / kBytesPerUs > .75f * compute_us && out > .5f * all && a.ldy * os % 64 == 0 && (uintptr_t)a.Y % 64 == 0;
 }
 
 static int choose_shape(ProductArgs& a, int64_t row_bytes, bool direct) {
@@ -877,12 +883,11 @@ static int choose_shape(ProductArgs& a, int64_t row_bytes, bool direct) {
         if (cost < least) { least = cost; best = i; }
     }
     // Where the bytes alone take longer than that, a copy's many small workgroups are best (100 000 rows, int8 127 -> 256: 33 us with 64 x 64,
-    // 41 .. 50 with the larger ones) - unless Y is stored past the caches, where whole 128-byte lines count, or nearly all of the bytes
-    // are weights of groups with few rows, which 128 x 128 reads more seldom (64 groups, 2 048 rows, 2 048 bytes x 1 024 columns: 28 us
-    // against 37 of 64 x 64).
+    // 41 .. 50 with the larger ones; 128 -> 256, Y past the caches: 24 against 31 .. 42) - unless nearly all of the bytes are weights of
+    // groups with few rows, which 128 x 128 reads more seldom (64 groups, 2 048 rows, 2 048 bytes x 1 024 columns: 28 us against 37).
     a.stream = streams_out(a, row_bytes, least);
     const float weights = weight_bytes(a, row_bytes), others = (float)a.rows * row_bytes + out_bytes(a);
-    if (a.stream || (weights + others) / kBytesPerUs > least) best = direct && (a.stream || (a.gptr && weights > 4.f * others)) ? 1 : 0;
+    if (a.stream || (weights + others) / kBytesPerUs > least) best = direct && a.gptr && weights > 4.f * others ? 1 : 0;
     return best;
 }
 
