@@ -218,7 +218,7 @@ __device__ __forceinline__ void finish(const ProductArgs& a, int64_t r, int n, c
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             x[i] += bias[i];
-            x[i] = x[i] > 0.f ? x[i] : relu ? 0.f : x[i] * slope;
+            x[i] = x[i] <= 0.f ? (relu ? 0.f : x[i] * slope) : x[i];  // (NaN stays NaN)
         }
     }
 #pragma unroll
@@ -531,7 +531,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int slots, in
     };
     if (live == HALVES) run(std::true_type{});
     else run(std::false_type{});
-    if (live == 0) return;
+    if (live <= 0) return;
     if constexpr (KIND == K_BF16) write_tiles<KIND, __bf16, TM, TN>(a, t, wm, n0 + wn, acc);
     else if constexpr (KIND == K_F16) write_tiles<KIND, _Float16, TM, TN>(a, t, wm, n0 + wn, acc);
     else if constexpr (KIND != K_I8) write_tiles<KIND, float, TM, TN>(a, t, wm, n0 + wn, acc);
@@ -947,18 +947,19 @@ static int product_dispatch(const char* family, int kind, ProductArgs& a, hipStr
 
 static bool known_dtype(int32_t d) { return d == DGCN_F32 || d == DGCN_BF16 || d == DGCN_F16; }
 static bool known_act(int32_t a) { return a == DGCN_ACT_LINEAR || a == DGCN_ACT_LEAKY_RELU || a == DGCN_ACT_RELU; }
-constexpr int kMaxExtent = 0x7fffffff - 1023;  // tile corners stay within 32 bits
+constexpr int kMaxExtent = 0x7fffffff - 1023;  // tile corners, and offsets within a row, stay within 32 bits
 constexpr int kMaxInt8Depth = 131071;  // 128 * 128 * cin stays below 2^31
 
-static int check_sizes(const char* who, int32_t rows, int32_t cin, int32_t ctot, bool has_h, int64_t ldh, int64_t ldy, int32_t act) {
+static int check_sizes(const char* who, int32_t rows, int32_t cin, int32_t ctot, int size, bool has_h, int64_t ldh, int64_t ldy, int32_t act) {
     if (rows < 0 || cin <= 0 || ctot <= 0 || (has_h && ldh < cin) || ldy < ctot) return fail(DGCN_ERR_ARG, "%s: bad sizes", who);
     if (!known_act(act)) return fail(DGCN_ERR_ARG, "%s: unknown activation %d", who, act);
     if (rows > kMaxExtent || ctot > kMaxExtent) return fail(DGCN_ERR_UNSUPPORTED, "%s: more than %d rows or columns", who, kMaxExtent);
+    if ((int64_t)cin * size > kMaxExtent) return fail(DGCN_ERR_UNSUPPORTED, "%s: rows of more than %d bytes", who, kMaxExtent);
     return DGCN_OK;
 }
 
 static int product_int8(const char* who, const char* family, ProductArgs& a, hipStream_t s) {
-    int rc = check_sizes(who, a.rows, a.cin, a.ctot, true, a.ldh, a.ldy, a.act);
+    int rc = check_sizes(who, a.rows, a.cin, a.ctot, 1, true, a.ldh, a.ldy, a.act);
     if (rc) return rc;
     if (!known_dtype(a.out_dtype)) return fail(DGCN_ERR_ARG, "%s: unknown dtype %d", who, a.out_dtype);
     if (a.cin > kMaxInt8Depth) return fail(DGCN_ERR_UNSUPPORTED, "%s: cin %d > %d: the int32 sums could overflow", who, a.cin, kMaxInt8Depth);
@@ -999,7 +1000,7 @@ extern "C" int dgcn_transform_grouped_batch(const void* H, int32_t dtype, int64_
                                             int32_t num_models, int32_t ctot, const float* bias, int32_t act, int32_t precise, void* Y,
                                             int64_t ldy, int32_t* status, void* stream) {
     const char* who = "dgcn_transform_grouped_batch";
-    int rc = check_sizes(who, rows, cin, ctot, H != nullptr, ldh, ldy, act);
+    int rc = check_sizes(who, rows, cin, ctot, dtype == DGCN_F32 ? 4 : 2, H != nullptr, ldh, ldy, act);
     if (rc) return rc;
     if (!known_dtype(dtype)) return fail(DGCN_ERR_ARG, "%s: unknown dtype %d", who, dtype);
     if (num_groups < 0 || num_models <= 0) return fail(DGCN_ERR_ARG, "%s: bad sizes", who);

@@ -114,6 +114,20 @@ def _matrix(x, what, dtypes, cols=None, rows=None):
     return ld
 
 
+def _overlap(x, ldx, y, ldy):
+    """Do two matrices share memory?  Column ranges of one buffer's rows do not."""
+    ax, ay, ex, ey = x.data_ptr(), y.data_ptr(), x.element_size(), y.element_size()
+    r, c = x.shape[-2:]
+    if x.dim() == 3:
+        r *= x.shape[0]
+    s, d = y.shape
+    if ax + ((r - 1) * ldx + c) * ex <= ay or ay + ((s - 1) * ldy + d) * ey <= ax or not r or not s:
+        return False
+    pitch = ldx * ex
+    off = (ay - ax) % max(pitch, 1)
+    return pitch != ldy * ey or off < c * ex or off + d * ey > pitch
+
+
 def _array(x, what, dtype, shape):
     """Check a contiguous tensor of one dtype and shape."""
     if x.dtype != dtype:
@@ -329,6 +343,8 @@ class Engine:
             out, ldy = self.torch.empty((rows, ctot), dtype=dtype, device=self.device), max(ctot, 1)
         else:
             ldy = _matrix(out, "out", (dtype,), cols=ctot, rows=rows)
+            if (H is not None and _overlap(H, ldh, out, ldy)) or _overlap(W, cin, out, ldy):
+                raise ValueError("out shares memory with H or the weights")
         self._here(H, W, bias, out)
         return rows, cin, ctot, M, ldh, ACT_CODES[act], codes[dtype], out, ldy
 
@@ -366,6 +382,8 @@ class Engine:
         else:
             q, scale = out
             ldq = _matrix(q, "q", (t.int8,), cols=cols, rows=rows)
+            if _overlap(X, ldx, q, ldq):
+                raise ValueError("q shares memory with X")
             _array(scale, "scale", t.float32, (rows,))
         self._here(X, q, scale)
         self._launch(self.lib.dgcn_quantize_rows_batch, "dgcn_quantize_rows_batch", X.data_ptr(), codes[X.dtype], ldx, rows, cols,
@@ -469,6 +487,7 @@ class Engine:
         objects with such ``.layers``, e.g. ``gcn.models.GCN_DQN``).  ``precision="int8"``: the products of the hidden layers run in 8-bit integers
         with scales per vertex and output column; the first and the last layer stay in float32 (as do all aggregations)."""
         t = self.torch
+        models = list(models)
         if any(getattr(m, "has_head", False) for m in models):
             raise _lib.DgcnError("a bank takes models whose output is their last layer (no is_dual / skip head)")
         models = [getattr(m, "layers", m) for m in models]
@@ -518,19 +537,22 @@ class Engine:
             return t.empty((0, bank.out_dim), dtype=t.float32, device=self.device)
         if x_const is None:
             x_const = float(np.float32(1.0 / bank.in_dim))
-        lap = self.supports(b, status=status)
-        H = X
-        for l, lyr in enumerate(bank.layers):
-            out = lyr["out"]
-            if lyr["q"] is not None:
-                q, s = self.quantize_rows(H)
-                Z = self.transform_grouped_int8(q, s, lyr["q"], lyr["scale"], b.graph_ptr, model_of_group=model_of_graph, bias=lyr["bias"],
-                                                status=status)
-            else:
-                Z = self.transform_grouped(H, lyr["weights"], b.graph_ptr, model_of_group=model_of_graph, bias=lyr["bias"], rows=n,
-                                           h_const=x_const, precise=l == 1, status=status)
-            H = self.spmm(lap, Z[:, out:], out, ldz=2 * out, graph_ptr=b.graph_ptr, num_graphs=B, max_nodes=b.host.max_nodes, Y0=Z,
-                          ldy0=2 * out, act=lyr["act"], precise=l == 0)
+        if b.lap is None and t.cuda.is_current_stream_capturing():
+            raise _lib.DgcnError("the batch's supports are made once and kept: call supports(b) before the capture")
+        with t.cuda.device(self._index()):
+            lap = self.supports(b, status=status)
+            H = X
+            for l, lyr in enumerate(bank.layers):
+                out = lyr["out"]
+                if lyr["q"] is not None:
+                    q, s = self.quantize_rows(H)
+                    Z = self.transform_grouped_int8(q, s, lyr["q"], lyr["scale"], b.graph_ptr, model_of_group=model_of_graph,
+                                                    bias=lyr["bias"], status=status)
+                else:
+                    Z = self.transform_grouped(H, lyr["weights"], b.graph_ptr, model_of_group=model_of_graph, bias=lyr["bias"], rows=n,
+                                               h_const=x_const, precise=l == 1, status=status)
+                H = self.spmm(lap, Z[:, out:], out, ldz=2 * out, graph_ptr=b.graph_ptr, num_graphs=B, max_nodes=b.host.max_nodes, Y0=Z,
+                              ldy0=2 * out, act=lyr["act"], precise=l == 0)
         if own:
             self.check_status(status)
         return H

@@ -236,11 +236,13 @@ int dgcn_transform_f64acc_batch(const float* H, int32_t ldh, float h_const, int3
  *    before the first and behind the last group are left as they were.  DGCN_FAULT_BAD_GROUP in *status (required; the caller
  *    zeroes it once): a pointer that decreases or leaves [0, rows], a model id outside [0, num_models) - that group's rows are
  *    left as they were (bad pointers: clamped, contents of Y's rows then undefined).
- *  - act is applied behind the bias.  Y / Q must not overlap the inputs.  No atomics but the status word, no workspace, nothing kept
- *    between calls: a row's result depends on that row, its model and the call's sizes, types and alignment only (float32: on the row
- *    and its model), and repeated calls return the same bits.
+ *    rows == 0 or num_groups == 0: nothing is launched, nothing reported.
+ *  - act is applied behind the bias; NaN stays NaN.  Y / Q must not overlap the inputs.  No atomics but the status word, no workspace,
+ *    nothing kept between calls: a row's result depends on that row, its model and the call's sizes, types and alignment only (float32:
+ *    on the row and its model), and repeated calls return the same bits.
  *  - Any alignment the element type has is taken; rows of H and W at multiples of 16 bytes are fastest (bytes at odd addresses: about half
- *    the rate).  DGCN_ERR_UNSUPPORTED: more than 2^31 - 1 024 rows or columns, or a call of more than some 2^24 tiles of 64 x 64.
+ *    the rate).  DGCN_ERR_UNSUPPORTED: more than 2^31 - 1 024 rows, columns or bytes of a row (cin), or a call of more than 2^24 output
+ *    tiles (32 x 64 at least where rows and columns are many).
  *
  * dgcn_quantize_rows_batch: Q[r][k] = x / scale[r] rounded half to even (exact quotient), |Q| <= 127;
  *   scale[r] = max(max_k |X[r][k]| / 127, 2^-126) in float32.  A row with a NaN or an infinity gets scale NaN and Q = 0, so that every

@@ -351,6 +351,23 @@ def test_non_finite_values_stay_in_their_row_and_column(engine):
             assert torch.equal(bad, want), (dtype, rows)
 
 
+@pytest.mark.parametrize("rows,cin,ctot", [(9, 64, 33), (40, 1024, 64), (300, 200, 130), (140000, 64, 16)])
+def test_nan_passes_every_activation(engine, rows, cin, ctot):
+    import torch
+    x = torch.randn(rows, cin, device="cuda:0", generator=_gen(3))
+    x[4, 5] = float("nan")
+    ptr, _ = _groups([rows])
+    W = torch.randn(1, ctot, cin, device="cuda:0", generator=_gen(4))
+    q, s = engine.quantize_rows(x)
+    wq, ws = engine.quantize_rows(W[0])
+    want = torch.zeros(rows, ctot, dtype=torch.bool, device="cuda:0")
+    want[4] = True
+    for act in ("linear", "leaky_relu", "relu"):
+        for y in (engine.transform_int8(q, s, wq, ws, act=act), engine.transform_grouped(x, W, ptr, act=act), engine.transform_grouped(x, W, ptr, act=act, precise=True),
+                  engine.transform_grouped(x.half(), W.half(), ptr, act=act)):
+            assert torch.equal(torch.isnan(y), want), act
+
+
 def test_bad_groups_are_reported_and_leave_their_rows(engine):
     import torch
     from distgcn_amd._lib import DgcnError
@@ -540,6 +557,38 @@ def test_int8_bank_is_the_written_formula(engine, hidden):
         y = engine.spmm(lap, z[:, 1:].contiguous(), 1, graph_ptr=db.graph_ptr, num_graphs=hb.num_graphs, max_nodes=hb.max_nodes, Y0=z, ldy0=2).cpu().numpy()
         want[of_row == m] = y[of_row == m]
     assert np.array_equal(scores, want)
+
+
+@pytest.mark.parametrize("precision", ["float32", "int8"])
+def test_captured_bank_follows_its_inputs(engine, precision):
+    """A whole forward pass in a graph: replays with other features and other models per graph, eager work between them."""
+    import torch
+    from distgcn_amd import datagen
+    from distgcn_amd._lib import DgcnError
+    hb, db, of, mog = _mixed_batch(engine)
+    bank = engine.model_bank([datagen.random_model(4, 24, feature_size=4, seed=i) for i in range(3)], precision=precision)
+    X = torch.randn(hb.num_nodes, 4, device="cuda:0", generator=_gen(1))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda:0")
+    with pytest.raises(DgcnError, match="before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.zeros(1, device="cuda:0")
+            engine.forward_bank(db, bank, mog, X=X, status=status)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        engine.forward_bank(db, bank, mog, X=X, status=status)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = engine.forward_bank(db, bank, mog, X=X, status=status)
+    for seed in range(4):
+        X.copy_(torch.randn(X.shape, device="cuda:0", generator=_gen(60 + seed)))
+        mog.copy_((mog + 1) % 3)
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, engine.forward_bank(db, bank, mog, X=X, status=status))
+        assert int(status) == 0
 
 
 def test_bank_reports_a_wrong_model_id(engine):

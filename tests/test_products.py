@@ -133,6 +133,37 @@ def test_python_refusals(host_engine):
         e.transform_int8(hq, hs, wq[0], ws[0], bias=z(4), act="relu", dtype=torch.bfloat16)
 
 
+def test_outputs_that_share_memory_are_refused(host_engine):
+    import torch
+    e = host_engine
+    ptr = torch.tensor([0, 2, 6], dtype=torch.int32)
+    buf = torch.zeros(6, 24)
+    H, W = buf[:, :8], torch.zeros(2, 8, 8)
+    for out in (H, buf[:, 4:12], buf.reshape(-1)[:48].reshape(6, 8), buf.reshape(-1)[20:68].reshape(6, 8), W.reshape(16, 8)[3:9]):
+        with pytest.raises(ValueError, match="shares memory"):
+            e.transform_grouped(H, W, ptr, out=out)
+    for out in (buf[:, 8:16], buf[:, 16:], torch.zeros(6, 8)):
+        with pytest.raises(AssertionError, match="accepted"):
+            e.transform_grouped(H, W, ptr, out=out)
+    q = buf.view(torch.int8)
+    with pytest.raises(ValueError, match="shares memory"):
+        e.quantize_rows(H, out=(q[:, 24:32], torch.zeros(6)))
+    with pytest.raises(AssertionError, match="accepted"):
+        e.quantize_rows(H, out=(q[:, 32:40], torch.zeros(6)))
+    h8 = q[:, :8]
+    with pytest.raises(ValueError, match="shares memory"):
+        e.transform_int8(h8, torch.zeros(6), torch.zeros(1, 8, dtype=torch.int8), torch.zeros(1), out=buf[:, 1:2])
+    with pytest.raises(AssertionError, match="accepted"):
+        e.transform_int8(h8, torch.zeros(6), torch.zeros(1, 8, dtype=torch.int8), torch.zeros(1), out=buf[:, 2:3])
+
+
+def test_rows_beyond_32_bit_offsets_are_refused(lib):
+    f, big = lib.dgcn_transform_grouped_batch, 600_000_000  # 2.4 GB of float32 a row
+    for dtype, cin in ((0, big), (0, 536870657), (1, 1073741313), (2, 0x7fffffff)):
+        rc = f(P, dtype, cin, 0.5, 4, cin, P, None, 2, P, 2, 8, None, 0, 0, P, 8, P, None)
+        _refused(lib, rc, -3, "bytes")
+
+
 def test_bank_refusals(host_engine):
     import numpy as np
     from distgcn_amd import datagen
