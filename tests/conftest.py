@@ -14,6 +14,15 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
 
 
+def pytest_collection_modifyitems(config, items):
+    """The tests that run the reference itself need its files: an empty folder in its place holds none."""
+    ref = os.environ.get("DGCN_REFERENCE", "/root/reference")
+    if not os.path.isfile(os.path.join(ref, "heuristics.py")):
+        for item in items:
+            if item.name in ("test_reference_import_agrees_when_available", "test_reference_execution_is_reproducible_when_available"):
+                item.add_marker(pytest.mark.skip(reason="reference tree not present"))
+
+
 class Golden:
     """Fixture data generated by oracle/make_golden.py from the imported reference."""
 
