@@ -96,7 +96,7 @@ class ModelBank:
 
 
 def _matrix(x, what, dtypes, cols=None, rows=None):
-    """Check a 2-D tensor whose rows are contiguous; -> its row stride in elements."""
+    """Check a 2-D tensor whose rows are contiguous; -> (rows, columns, row stride in elements)."""
     if x.dtype not in dtypes:
         raise TypeError("%s is %s, expected %s" % (what, x.dtype, " / ".join(str(d) for d in dtypes)))
     shape = x.shape
@@ -108,10 +108,10 @@ def _matrix(x, what, dtypes, cols=None, rows=None):
     if inner != 1 and c > 1:
         raise ValueError("%s: the entries of a row must be contiguous" % what)
     if r <= 1:
-        return max(c, 1)
+        return r, c, max(c, 1)
     if ld < c:
         raise ValueError("%s: rows overlap (row stride %d, %d columns)" % (what, ld, c))
-    return ld
+    return r, c, ld
 
 
 def _overlap(x, ldx, y, ldy):
@@ -321,40 +321,39 @@ class Engine:
             _lib.check(rc, what)
 
     def _product_args(self, H, W, bias, act, dtype, out, grouped, rows=None):
-        """The checks every product shares -> (rows, cin, ctot, models, ldh, activation code, dtype code, out, ldy)."""
+        """The checks every product shares, but for the device -> (rows, cin, ctot, models, ldh, activation code, dtype code, out, ldy)."""
         codes = self._codes
         if dtype not in codes:
             raise TypeError("dtype is %s, expected %s" % (dtype, " / ".join(str(d) for d in codes)))
         if act not in ACT_CODES:
             raise ValueError("unknown activation %r" % (act,))
-        if W.dim() != (3 if grouped else 2):
-            raise ValueError("the weights have shape %s, expected %s" % (tuple(W.shape), "[models, ctot, cin]" if grouped else "[ctot, cin]"))
+        shape = W.shape
+        if len(shape) != (3 if grouped else 2):
+            raise ValueError("the weights have shape %s, expected %s" % (tuple(shape), "[models, ctot, cin]" if grouped else "[ctot, cin]"))
         if not W.is_contiguous():
             raise ValueError("the weights must be contiguous")
-        ctot, cin = W.shape[-2], W.shape[-1]
-        M = W.shape[0] if grouped else 1
+        M, ctot, cin = shape if grouped else (1, *shape)
         ldh = cin
         if H is not None:
-            ldh = _matrix(H, "H", (W.dtype,), cols=cin, rows=rows)
-            rows = H.shape[0]
+            rows, _, ldh = _matrix(H, "H", (W.dtype,), cols=cin, rows=rows)
         if bias is not None:
             _array(bias, "bias", self.torch.float32, (M, ctot) if grouped else (ctot,))
         if out is None:
             out, ldy = self.torch.empty((rows, ctot), dtype=dtype, device=self.device), max(ctot, 1)
         else:
-            ldy = _matrix(out, "out", (dtype,), cols=ctot, rows=rows)
+            ldy = _matrix(out, "out", (dtype,), cols=ctot, rows=rows)[2]
             if (H is not None and _overlap(H, ldh, out, ldy)) or _overlap(W, cin, out, ldy):
                 raise ValueError("out shares memory with H or the weights")
-        self._here(H, W, bias, out)
         return rows, cin, ctot, M, ldh, ACT_CODES[act], codes[dtype], out, ldy
 
     def _groups(self, group_ptr, model_of_group, num_models, status):
         """The arguments every grouped product shares -> (number of groups, status word, is the word this call's own)."""
         t = self.torch
-        if group_ptr.dim() != 1 or group_ptr.numel() < 1:
-            raise ValueError("group_ptr has shape %s, expected [groups + 1]" % (tuple(group_ptr.shape),))
-        G = group_ptr.numel() - 1
-        _array(group_ptr, "group_ptr", t.int32, (G + 1,))
+        shape = group_ptr.shape
+        if len(shape) != 1 or shape[0] < 1:
+            raise ValueError("group_ptr has shape %s, expected [groups + 1]" % (tuple(shape),))
+        G = shape[0] - 1
+        _array(group_ptr, "group_ptr", t.int32, shape)
         if model_of_group is not None:
             _array(model_of_group, "model_of_group", t.int32, (G,))
         elif num_models < G:
@@ -374,14 +373,13 @@ class Engine:
         a row with a NaN or an infinity gets scale NaN."""
         t = self.torch
         codes = self._codes
-        ldx = _matrix(X, "X", codes)
-        rows, cols = X.shape
+        rows, cols, ldx = _matrix(X, "X", codes)
         if out is None:
             q, scale = t.empty((rows, cols), dtype=t.int8, device=self.device), t.empty(rows, dtype=t.float32, device=self.device)
             ldq = max(cols, 1)
         else:
             q, scale = out
-            ldq = _matrix(q, "q", (t.int8,), cols=cols, rows=rows)
+            ldq = _matrix(q, "q", (t.int8,), cols=cols, rows=rows)[2]
             if _overlap(X, ldx, q, ldq):
                 raise ValueError("q shares memory with X")
             _array(scale, "scale", t.float32, (rows,))
@@ -401,7 +399,7 @@ class Engine:
             Hq, Wq, bias, act, dtype or (t.float32 if out is None else out.dtype), out, False)
         _array(h_scale, "h_scale", t.float32, (rows,))
         _array(w_scale, "w_scale", t.float32, (ctot,))
-        self._here(h_scale, w_scale)
+        self._here(Hq, Wq, h_scale, w_scale, bias, out)
         self._launch(self.lib.dgcn_transform_int8_batch, "dgcn_transform_int8_batch", Hq.data_ptr(), ldh, h_scale.data_ptr(), rows, cin,
                      Wq.data_ptr(), w_scale.data_ptr(), ctot, None if bias is None else bias.data_ptr(), code, out.data_ptr(), dt, ldy)
         return out
@@ -420,6 +418,7 @@ class Engine:
         if precise and W.dtype != t.float32:
             raise ValueError("precise takes float32")
         rows, cin, ctot, M, ldh, code, dt, out, ldy = self._product_args(H, W, bias, act, W.dtype, out, True, rows)
+        self._here(H, W, bias, out)
         G, status, own = self._groups(group_ptr, model_of_group, M, status)
         self._launch(self.lib.dgcn_transform_grouped_batch, "dgcn_transform_grouped_batch", None if H is None else H.data_ptr(), dt, ldh,
                      float(h_const), rows, cin, group_ptr.data_ptr(), None if model_of_group is None else model_of_group.data_ptr(), G,
@@ -440,7 +439,7 @@ class Engine:
             Hq, Wq, bias, act, dtype or (t.float32 if out is None else out.dtype), out, True)
         _array(h_scale, "h_scale", t.float32, (rows,))
         _array(w_scale, "w_scale", t.float32, (M, ctot))
-        self._here(h_scale, w_scale)
+        self._here(Hq, Wq, h_scale, w_scale, bias, out)
         G, status, own = self._groups(group_ptr, model_of_group, M, status)
         self._launch(self.lib.dgcn_transform_grouped_int8_batch, "dgcn_transform_grouped_int8_batch", Hq.data_ptr(), ldh,
                      h_scale.data_ptr(), rows, cin, group_ptr.data_ptr(), None if model_of_group is None else model_of_group.data_ptr(), G,
