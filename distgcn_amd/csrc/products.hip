@@ -36,6 +36,7 @@ struct ProductArgs {
     int rows, cin, ctot, num_groups, num_models, act, out_dtype;
     bool dwords_h, dwords_w;  // rows of H, of W start at multiples of 4 bytes
     bool stream;              // Y is stored past the caches (see streams_out)
+    bool counted;             // tiles are numbered by find_tile_counted
 };
 
 template <int KIND> struct Elem;
@@ -68,7 +69,7 @@ __device__ __forceinline__ bool bad_group(const ProductArgs& a, int p0, int p1, 
     return p0 < 0 || p1 < p0 || p1 > a.rows || e < 0 || e >= a.num_models;
 }
 
-// Up to 256 groups: every wave reads the whole table, four groups per lane, and counts their row tiles, so that every workgroup up to
+// Up to 256 groups and rows of more than 256 bytes (see product_dispatch): every wave reads the whole table, four groups per lane, and counts their row tiles, so that every workgroup up to
 // the number of tiles has one (at most min(rows, floor(rows / BM) + num_groups) x column tiles) and the XCDs' shares are equal.  A
 // group's tiles are neighbours, column by column: its weights are read into an XCD's L2 once (64 groups of 256 rows on average, int8
 // 2 000 x 2 050: with the groups' last, shorter tiles numbered behind all others 654 MB passed the L2 instead of 448).  Workgroup 0
@@ -127,11 +128,11 @@ template <int BM> __device__ __forceinline__ Tile find_tile_counted(const Produc
     return t;
 }
 
-// More groups: no count at all.  Group g's row tiles start at slot floor(p_g / BM) + g, which is increasing in g, and
+// Otherwise no count at all.  Group g's row tiles start at slot floor(p_g / BM) + g, which is increasing in g, and
 // ceil((p_{g+1} - p_g) / BM) never exceeds the distance to the next group's start.  So floor(rows / BM) + num_groups slots cover every
 // tile (some slots are empty), and a slot finds its group by search: 64-ary, a lane per probe.  Slot g < num_groups checks entry g.
 template <int BM> __device__ __forceinline__ Tile find_tile(const ProductArgs& a, int b, int slots, int col_tiles) {
-    if (a.gptr && a.num_groups <= kCountedGroups) return find_tile_counted<BM>(a, b, col_tiles);
+    if (a.counted) return find_tile_counted<BM>(a, b, col_tiles);
     Tile t{0, 0, 0, 0};
     const int slot = patch_order(xcd_order(b, slots * col_tiles), slots, col_tiles, t.col);
     if (!a.gptr) {
@@ -323,7 +324,18 @@ __device__ __forceinline__ i32x4 load_chunk(const char* row, int64_t off, int64_
     return i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
 }
 
-// The same for a chunk that lies at least 16 bytes behind its row's start and ends at least 4 bytes in front of its end, in rows that
+// A row's last 16 bytes -> the chunk that starts `by` bytes behind their start (by <= 0: it is whole already): zeros move in.
+__device__ __forceinline__ i32x4 shift_chunk(i32x4 v, int by) {
+    by = min(max(by, 0), 16);
+    const bool two = by & 8, one = by & 4;
+    int a = two ? v[2] : v[0], b = two ? v[3] : v[1], c = two ? 0 : v[2], d = two ? 0 : v[3];
+    a = one ? b : a; b = one ? c : b; c = one ? d : c; d = one ? 0 : d;
+    if (by == 16) a = b = c = d = 0;
+    return i32x4{(int)__builtin_amdgcn_alignbyte(b, a, by & 3), (int)__builtin_amdgcn_alignbyte(c, b, by & 3), (int)__builtin_amdgcn_alignbyte(d, c, by & 3),
+                 (int)__builtin_amdgcn_alignbyte(0, d, by & 3)};
+}
+
+// load_chunk for a chunk that lies at least 16 bytes behind its row's start and ends at least 4 bytes in front of its end, in rows that
 // start at any byte: five aligned dwords, shifted by the address' low bits.  (A 16-byte load from an address that is no multiple of 4
 // takes several times as long.)
 struct Dwords { i32x4 v; int v4; };
@@ -426,17 +438,23 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int slots, in
                 }
             }
         } else {
+            auto no_h = [&](int i) { return (KIND == K_F32 || KIND == K_F32P) && i < NH && !a.H; };  // (there is no H: h_const)
 #pragma unroll
             for (int i = 0; i < NH + NW; ++i) {
                 if (W_PART && i == NH + NW - 1 && (i - NH) * T + wave * 64 >= BN * 8) continue;
-                if ((KIND == K_F32 || KIND == K_F32P) && i < NH && !a.H) {
+                if (no_h(i)) {
 #pragma unroll
                     for (int x = 0; x < 4; ++x) reg[i][x] = at + koff[i] + 4 * x < kbytes ? __builtin_bit_cast(int, a.h_const) : 0;
-                } else if (whole) {
-                    __builtin_memcpy(&reg[i], src[i] + at + koff[i], 16);
+                } else if (kbytes >= 16) {  // (the row's last 16 bytes for a chunk that crosses its end)
+                    __builtin_memcpy(&reg[i], src[i] + (whole ? at + koff[i] : min(at + koff[i], (int)kbytes - 16)), 16);
                 } else {
                     reg[i] = load_chunk(src[i], at + koff[i], kbytes);
                 }
+            }
+            if (!whole && kbytes >= 16) {
+#pragma unroll
+                for (int i = 0; i < NH + NW; ++i)
+                    if (!no_h(i)) reg[i] = shift_chunk(reg[i], at + koff[i] - ((int)kbytes - 16));
             }
         }
     };
@@ -543,8 +561,10 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int slots, in
     else write_tiles<KIND, float, TM, TN>(a, t, wm, n0 + wn, acc);
 }
 
+// (Stages through registers: five waves per SIMD for the small tiles, not the four that the compiler would choose - short rows are latency:
+// 79 002 rows, bf16 30 -> 380 in 378 groups 47 -> 36 us, 100 000 rows int8 127 -> 256 float32 36 -> 30.)
 template <int KIND, int BM, int BN, int WM, int WN, int NBUF, bool DIRECT>
-__global__ __launch_bounds__(WM* WN * 64) void k_product(ProductArgs a, int slots, int col_tiles) {
+__global__ __launch_bounds__(WM* WN * 64, !DIRECT && WM * WN == 4 && BN == 64 && KIND != K_F32P ? 5 : 1) void k_product(ProductArgs a, int slots, int col_tiles) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     product_tile<KIND, BM, BN, WM, WN, NBUF, DIRECT>(a, slots, col_tiles, smem);
 }
@@ -774,7 +794,7 @@ __global__ __launch_bounds__(256) void k_product_rows(ProductArgs a, int run) { 
 static int64_t row_slots(const ProductArgs& a, int BM) {
     if (!a.gptr) return ((int64_t)a.rows + BM - 1) / BM;
     const int64_t n = (int64_t)a.rows / BM + a.num_groups;
-    return a.num_groups <= kCountedGroups ? min(n, (int64_t)a.rows) : n;  // (a counted tile holds at least one row)
+    return a.counted ? min(n, (int64_t)a.rows) : n;  // (a counted tile holds at least one row)
 }
 constexpr int64_t max_grid(int threads) { return 0xffffffffu / (unsigned)threads; }  // a launch's threads are counted in 32 bits
 
@@ -886,8 +906,8 @@ static int choose_shape(ProductArgs& a, int64_t row_bytes, bool direct) {
         if (rest > .02f) cost += (p.s1 + (p.per_cu > 1 ? (p.sc - p.s1) * (ceilf(rest) - 1.f) / (p.per_cu - 1) : 0.f)) * steps + p.f;
         if (cost < least) { least = cost; best = i; }
     }
-    // Where the bytes alone take longer than that, a copy's many small workgroups are best (100 000 rows, int8 127 -> 256: 33 us with 64 x 64,
-    // 41 .. 50 with the larger ones; 128 -> 256, Y past the caches: 24 against 31 .. 42) - unless nearly all of the bytes are weights of
+    // Where the bytes alone take longer than that, a copy's many small workgroups are best (100 000 rows, int8 127 -> 256: 33 us with 64 x 64
+    // when the larger ones took 41 .. 50; 128 -> 256, Y past the caches: 24 against 31 .. 42) - unless nearly all of the bytes are weights of
     // groups with few rows, which 128 x 128 reads more seldom (64 groups, 2 048 rows, 2 048 bytes x 1 024 columns: 28 us against 37).
     a.stream = streams_out(a, row_bytes, least);
     const float weights = weight_bytes(a, row_bytes), others = (float)a.rows * row_bytes + out_bytes(a);
@@ -938,6 +958,9 @@ template <int KIND> static int dispatch_kind(const char* family, ProductArgs& a,
 
 static int product_dispatch(const char* family, int kind, ProductArgs& a, hipStream_t s) {
     const int es = kind == K_I8 ? 1 : kind == K_BF16 || kind == K_F16 ? 2 : 4;
+    // Counting pays where a tile is long (16 000 rows of 1 024 bytes in 64 groups, 512 columns, int8: 20 us, searching 31; of 4 096 bytes 58
+    // against 91); in short ones its loads are a part of the time (40 000 rows of 128 bytes in 8 groups: 20 against 17; in 250: 29 against 25).
+    a.counted = a.gptr && a.num_groups <= kCountedGroups && (int64_t)a.cin * es > 256;
     a.dwords_h = (uintptr_t)a.H % 4 == 0 && a.ldh * es % 4 == 0;
     a.dwords_w = (uintptr_t)a.W % 4 == 0 && (int64_t)a.cin * es % 4 == 0;
     switch (kind) {
