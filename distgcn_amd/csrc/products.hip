@@ -270,8 +270,10 @@ template <int KIND> __device__ __forceinline__ int w_row(int i, int j, bool pair
     if constexpr (KIND == K_F32P) return j * 16 + 4 * (i & 3) + (i >> 2);
     else return pairs ? (j >> 1) * 32 + (i >> 2) * 8 + (j & 1) * 4 + (i & 3) : j * 16 + i;
 }
-// The chunk permutation of an LDS row of W: eight lanes in a row read eight different bank groups.
-__device__ __forceinline__ int w_key(int row, bool pairs) { return pairs ? (row & 3) | ((row >> 1) & 4) : row & 7; }
+// The chunk permutation of an LDS row: 16-byte reads - eight lanes in a row read eight different bank groups; dword reads - sixteen rows'
+// dwords lie in sixty-four different banks.
+template <int KIND> __device__ __forceinline__ int h_key(int row) { return KIND == K_F32 || KIND == K_F32P ? (row >> 1) & 7 : row & 7; }
+template <int KIND> __device__ __forceinline__ int w_key(int row, bool pairs) { return pairs ? (row & 3) | ((row >> 1) & 4) : h_key<KIND>(row); }
 
 // One wave's TM x TN tiles.
 template <int KIND, class O, int TM, int TN>
@@ -403,7 +405,7 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int slots, in
     for (int i = 0; i < NH + NW; ++i) {
         const bool is_h = i < NH;
         const int c = (is_h ? i : i - NH) * T + tid, row = c >> 3;
-        koff[i] = ((c & 7) ^ (is_h ? row & 7 : w_key(row, pairs))) << 4;
+        koff[i] = ((c & 7) ^ (is_h ? h_key<KIND>(row) : w_key<KIND>(row, pairs))) << 4;
         const int last = is_h ? t.row1 - 1 - t.row0 : a.ctot - 1 - n0;
         const int64_t stride = is_h ? a.ldh * ES : kbytes;
         if constexpr (DIRECT) at0[i] = min(row, last) * (int)stride + koff[i];
@@ -480,11 +482,11 @@ __device__ __forceinline__ void product_tile(const ProductArgs& a, int slots, in
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
                 const int row = w_row<KIND>(lane & 15, j, pairs);
-                fw[AHEAD ? k : 0][j] = lds_frag<KIND, RB>(sW, wn + row, w_key(row, pairs), k);
+                fw[AHEAD ? k : 0][j] = lds_frag<KIND, RB>(sW, wn + row, w_key<KIND>(row, pairs), k);
             }
         }
 #pragma unroll
-        for (int i = 0; i < RT; ++i) fh[AHEAD ? p & 1 : 0][i] = lds_frag<KIND, RB>(sH, wm + (half * RT + i) * 16 + (lane & 15), lane & 7, k);
+        for (int i = 0; i < RT; ++i) fh[AHEAD ? p & 1 : 0][i] = lds_frag<KIND, RB>(sH, wm + (half * RT + i) * 16 + (lane & 15), h_key<KIND>(lane & 15), k);
     };
     auto multiply_rows = [&](int p, int from, int to) {
         const int k = p / HALVES, half = p % HALVES;
