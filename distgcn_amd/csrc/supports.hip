@@ -34,10 +34,12 @@ __global__ __launch_bounds__(256) void k_supports(const int32_t* __restrict__ gr
         if (v == num_nodes - 1) lap_row_ptr[num_nodes] = re + num_nodes;
     }
     for (int j = rs + sub; j < re; j += 8) {
-        const int u = col_idx[j];
+        int u = col_idx[j];
         float val = 0.0f;
         if (u < n0 || u >= n1) {
+            // (the aggregations behind this launch are not told of the fault: 0 times the row itself keeps them inside the matrix)
             fault |= DGCN_FAULT_BAD_COLUMN;
+            u = v;
         } else {
             if (u == v) fault |= DGCN_FAULT_SELF_LOOP;
             const int du = row_ptr[u + 1] - row_ptr[u];

@@ -165,7 +165,8 @@ int dgcn_expand_compact_batch(const void* compact_dev, const DgcnCompactInfo* co
  * reference's); each off-diagonal is (float)(-(dinv[deg u] * dinv[deg v])), the diagonal 1.0f -
  * exactly the float32 the reference feeds TF after its float64 -> float32 cast.
  * Outputs (caller-allocated): lap_row_ptr[num_nodes+1], lap_col[num_edges+num_nodes],
- * lap_val[num_edges+num_nodes].  Faults: SELF_LOOP, DEGREE_RANGE, BAD_COLUMN. */
+ * lap_val[num_edges+num_nodes].  Faults: SELF_LOOP, DEGREE_RANGE, BAD_COLUMN (the entry becomes 0 in its own row's column, so that
+ * aggregations over the result stay inside their matrices). */
 int dgcn_supports_batch(const DgcnBatch* batch, const double* dinv_table, int32_t table_len,
                         int32_t* lap_row_ptr, int32_t* lap_col, float* lap_val,
                         int32_t* status, void* stream);

@@ -1,0 +1,66 @@
+"""GPU: batches of several models when something is wrong with the batch - what is reported, how often, and what the launches behind the
+report may touch."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _graphs(sizes, seed):
+    import scipy.sparse as sp
+    rng = np.random.default_rng(seed)
+    adjs = []
+    for n in sizes:
+        a = np.triu(rng.random((n, n)) < min(1.0, 12.0 / max(n, 1)), 1)
+        adjs.append(sp.csr_matrix((a + a.T).astype(float)))
+    return adjs, [rng.random(n) for n in sizes]
+
+
+def _batch_with_columns(sizes, seed, where):
+    """A batch whose entries ``where`` = {(graph, entry of the graph): column id of the batch} point elsewhere."""
+    from distgcn_amd.batch import HostBatch
+    good = HostBatch.from_scipy(*_graphs(sizes, seed))
+    col = good.col_idx.copy()
+    for (g, e), c in where.items():
+        col[good.row_ptr[good.graph_ptr[g]] + e] = c
+    return good, HostBatch(good.graph_ptr, good.row_ptr, col, good.weights)
+
+
+FAR = {(1, 0): 2 ** 31 - 1, (1, 5): -1, (1, 9): -(2 ** 31), (3, 2): 0, (3, 40): 10 ** 6}
+
+
+@pytest.mark.parametrize("sizes", [[30, 50, 20, 70], [200, 900, 100, 300]])
+def test_columns_outside_their_graph_are_reported_and_never_followed(engine, sizes):
+    import torch
+    from distgcn_amd import datagen
+    from distgcn_amd._lib import DgcnError
+    from distgcn_amd.engine import DeviceModel
+    good, bad = _batch_with_columns(sizes, 1, FAR)
+    ok = [(lo, hi) for g, (lo, hi) in enumerate(good.graph_slices()) if g not in (1, 3)]
+    models = [datagen.random_model(3, 16, seed=s) for s in (1, 2)]
+    mog = torch.tensor([0, 1, 1, 0], dtype=torch.int32, device="cuda:0")
+    bank, dm = engine.model_bank(models), DeviceModel(models[0], "cuda:0")
+
+    status = torch.zeros(1, dtype=torch.int32, device="cuda:0")
+    lap = engine.supports(engine.upload(bad), status=status)
+    assert int(status) == 8
+    col, val, row = (lap[k].cpu().numpy() for k in ("col_idx", "values", "row_ptr"))
+    own = np.repeat(np.arange(bad.num_nodes), np.diff(row))
+    graph = np.repeat(np.arange(4), sizes)
+    assert np.array_equal(graph[col], graph[own])
+    for (g, e), c in FAR.items():
+        at = good.row_ptr[good.graph_ptr[g]] + e
+        at += int(np.searchsorted(good.row_ptr, at, side="right"))  # a diagonal entry in front of every row
+        assert col[at] == own[at] and val[at] == 0
+
+    with pytest.raises(DgcnError, match="column index"):
+        engine.forward_bank(engine.upload(bad), bank, mog)
+    clean = engine.solve_bank(engine.upload(good), bank, mog)
+    res = engine.solve_bank(engine.upload(bad), bank, mog)
+    assert int(clean["status"]) == 0 and int(res["status"]) & 8
+    one = engine.solve(engine.upload(bad), dm)
+    assert int(one["status"]) & 8
+    one_clean = engine.solve(engine.upload(good), dm)
+    for lo, hi in ok:  # the other graphs of the batch are what they are without it
+        for a, b in ((res, clean), (one, one_clean)):
+            assert torch.equal(a["scores"][lo:hi], b["scores"][lo:hi]) and torch.equal(a["state"][lo:hi], b["state"][lo:hi])
