@@ -71,6 +71,10 @@ __global__ __launch_bounds__(BLOCK) void k_lgs(LgsArgs a) {
     const int e0 = a.row_ptr[n0], e1 = a.row_ptr[n1];
     const bool cols_lds = (e1 - e0) <= a.cols_cap && ng <= 65536;
     for (int v = threadIdx.x; v <= ng; v += BLOCK) rol[v] = a.row_ptr[n0 + v];  // row bounds: read once, not per round
+    const bool ahead = !STATS && cols_lds && a.max_rounds <= 0 && ng <= 4096 && a.ahead_rounds;
+    // columns outside the graph (reported where the batch is validated): the ahead lists leave them out, the plain rounds take the
+    // last vertex instead, so that no index leaves the graph's arrays
+    const unsigned far = ahead ? 0xffffu : (unsigned)(ng - 1);
     if (cols_lds) {
         for (int base = e0 + threadIdx.x; base < e1; base += BLOCK * 4) {  // 4 loads in flight per thread
             int c[4];
@@ -78,7 +82,7 @@ __global__ __launch_bounds__(BLOCK) void k_lgs(LgsArgs a) {
             for (int i = 0; i < 4; ++i) c[i] = (base + i * BLOCK < e1) ? a.col_idx[base + i * BLOCK] : 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (base + i * BLOCK < e1) cl[base + i * BLOCK - e0] = (uint16_t)(c[i] - n0);
+                if (base + i * BLOCK < e1) cl[base + i * BLOCK - e0] = (uint16_t)min((unsigned)(c[i] - n0), far);
         }
     }
     if (a.cand) {  // this instance's start: the candidate and its neighbours do not take part
@@ -101,7 +105,7 @@ __global__ __launch_bounds__(BLOCK) void k_lgs(LgsArgs a) {
         for (int v = threadIdx.x; v < ng; v += BLOCK) a.state[n0 + v] = a.init_state ? a.init_state[n0 + v] : (uint8_t)0;
         return;
     }
-    if (!STATS && cols_lds && a.max_rounds <= 0 && ng <= 4096 && a.ahead_rounds) {
+    if (ahead) {
         // a whole search without statistics: the rounds on ahead lists (lgs_rounds.h: two walks over state / flag bytes per round;
         // the 16-bit counts in the reduction array's space, free until the totals)
         const int rounds = lgs_rounds_ahead<BLOCK, false>(ng, e0, pr, st, nw, cl, rol, reinterpret_cast<uint16_t*>(red), acc64);

@@ -38,10 +38,11 @@ struct LgsArgs {
     int ahead_rounds;           // whole searches without statistics: lgs_rounds_ahead below (0: lgs_rounds; option "wide_ahead" = 0)
 };
 
+// (a column outside the graph - reported where the batch is validated - reads the last vertex: no index leaves the graph's arrays)
 template <bool COLS_LDS>
-__device__ __forceinline__ int nbr_at(const uint16_t* cl, const int32_t* cg, int j, int e0, int n0) {
+__device__ __forceinline__ int nbr_at(const uint16_t* cl, const int32_t* cg, int j, int e0, int n0, int ng) {
     if (COLS_LDS) return cl[j - e0];
-    return cg[j] - n0;
+    return (int)min((unsigned)(cg[j] - n0), (unsigned)(ng - 1));
 }
 
 // One residual neighbour test: liveness byte, then the float64 priority compare of the total order
@@ -93,17 +94,17 @@ __device__ __forceinline__ void lgs_rounds(const LgsArgs& a, int g, int n0, int 
                 const int rs = ro[v], re = ro[v + 1];
                 int j = rs + sub;
                 for (; j + 3 * LPV < re; j += 4 * LPV) {  // four independent neighbour chains in flight
-                    const int u0 = nbr_at<COLS_LDS>(cl, a.col_idx, j, e0, n0);
-                    const int u1 = nbr_at<COLS_LDS>(cl, a.col_idx, j + LPV, e0, n0);
-                    const int u2 = nbr_at<COLS_LDS>(cl, a.col_idx, j + 2 * LPV, e0, n0);
-                    const int u3 = nbr_at<COLS_LDS>(cl, a.col_idx, j + 3 * LPV, e0, n0);
+                    const int u0 = nbr_at<COLS_LDS>(cl, a.col_idx, j, e0, n0, ng);
+                    const int u1 = nbr_at<COLS_LDS>(cl, a.col_idx, j + LPV, e0, n0, ng);
+                    const int u2 = nbr_at<COLS_LDS>(cl, a.col_idx, j + 2 * LPV, e0, n0, ng);
+                    const int u3 = nbr_at<COLS_LDS>(cl, a.col_idx, j + 3 * LPV, e0, n0, ng);
                     nbr_test(u0, v, pv, st, pr, lost, resid);
                     nbr_test(u1, v, pv, st, pr, lost, resid);
                     nbr_test(u2, v, pv, st, pr, lost, resid);
                     nbr_test(u3, v, pv, st, pr, lost, resid);
                 }
                 for (; j < re; j += LPV)
-                    nbr_test(nbr_at<COLS_LDS>(cl, a.col_idx, j, e0, n0), v, pv, st, pr, lost, resid);
+                    nbr_test(nbr_at<COLS_LDS>(cl, a.col_idx, j, e0, n0, ng), v, pv, st, pr, lost, resid);
             }
             if (LPV > 1) {
                 const unsigned long long m = __ballot(lost);
@@ -129,7 +130,7 @@ __device__ __forceinline__ void lgs_rounds(const LgsArgs& a, int g, int n0, int 
             if (v < ng && st[v] == 0 && nw[v]) {
                 const int rs = ro[v], re = ro[v + 1];
                 for (int j = rs + sub; j < re; j += LPV) {
-                    const int u = nbr_at<COLS_LDS>(cl, a.col_idx, j, e0, n0);
+                    const int u = nbr_at<COLS_LDS>(cl, a.col_idx, j, e0, n0, ng);
                     if (st[u] == 0) st[u] = 2;  // same value from every writer: benign
                 }
             }

@@ -64,3 +64,29 @@ def test_columns_outside_their_graph_are_reported_and_never_followed(engine, siz
     for lo, hi in ok:  # the other graphs of the batch are what they are without it
         for a, b in ((res, clean), (one, one_clean)):
             assert torch.equal(a["scores"][lo:hi], b["scores"][lo:hi]) and torch.equal(a["state"][lo:hi], b["state"][lo:hi])
+
+
+@pytest.mark.parametrize("kw", [{}, {"want_stats": True}, {"max_rounds": 1}])
+@pytest.mark.parametrize("sizes,degree", [([30, 50, 20, 70], 12), ([20, 2000, 30, 100], 80)])
+def test_greedy_search_stays_inside_its_graph(engine, sizes, degree, kw):
+    """Columns outside the graph, with the columns in LDS and - 2 000 vertices of 80 neighbours - in global memory."""
+    import torch
+    import scipy.sparse as sp
+    from distgcn_amd.batch import HostBatch
+    rng = np.random.default_rng(4)
+    adjs = []
+    for n in sizes:
+        a = np.triu(rng.random((n, n)) < min(1.0, degree / n), 1)
+        adjs.append(sp.csr_matrix((a + a.T).astype(float)))
+    good = HostBatch.from_scipy(adjs, [rng.random(n) for n in sizes])
+    col = good.col_idx.copy()
+    for (g, e), c in FAR.items():
+        col[good.row_ptr[good.graph_ptr[g]] + e] = c
+    bad = HostBatch(good.graph_ptr, good.row_ptr, col, good.weights)
+    prio = torch.from_numpy(rng.random(good.num_nodes)).cuda()
+    a, b = engine.lgs(engine.upload(good), prio=prio, **kw), engine.lgs(engine.upload(bad), prio=prio, **kw)
+    for g, (lo, hi) in enumerate(good.graph_slices()):
+        state = b["state"][lo:hi]
+        assert int(state.max()) <= 2 and (kw.get("max_rounds") or int(state.min()) >= 1)
+        if g in (0, 2):
+            assert torch.equal(state, a["state"][lo:hi]) and int(a["rounds"][g]) == int(b["rounds"][g])
