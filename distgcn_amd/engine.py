@@ -208,55 +208,77 @@ class Engine:
 
     # ------------------------------------------------------------------ A1/A2
     def supports(self, b: DeviceBatch, status=None):
-        """L = I - D^-1/2 A D^-1/2 for the batch (gcn/utils.py:258-274, k=1).  Cached on the batch."""
+        """L = I - D^-1/2 A D^-1/2 for the batch (gcn/utils.py:258-274, k=1).  Made once and kept with the batch, with the faults of its
+        adjacency: every call ORs them into ``status``, or raises without one (a call in a stream capture cannot: read
+        the word of the call that made them)."""
+        if b.lap is None:
+            lap = self._make_supports(b)
+            if status is None:
+                self.check_status(lap["faults"])
+                lap["checked"] = True
+            b.lap = lap
+        return self._kept(b.lap, status)
+
+    def _make_supports(self, b: DeviceBatch):
         t = self.torch
-        if b.lap is not None:
-            return b.lap
         n, e = b.host.num_nodes, b.host.num_edges
         row_ptr = t.empty(n + 1, dtype=t.int32, device=self.device)
         col = t.empty(max(n + e, 1), dtype=t.int32, device=self.device)
         val = t.empty(max(n + e, 1), dtype=t.float32, device=self.device)
-        own = status is None
-        if own:
-            status = t.zeros(1, dtype=t.int32, device=self.device)
+        faults = t.zeros(1, dtype=t.int32, device=self.device)
         tab = self._dinv(b.host.max_degree)
         if n == 0:
             row_ptr.zero_()
         _lib.check(self.lib.dgcn_supports_batch(C.byref(b.c), tab.data_ptr(), int(tab.numel()), row_ptr.data_ptr(),
-                                                col.data_ptr(), val.data_ptr(), status.data_ptr(), self._stream()),
+                                                col.data_ptr(), val.data_ptr(), faults.data_ptr(), self._stream()),
                    "dgcn_supports_batch")
-        if own:
-            self.check_status(status)
         csr = _lib.DgcnCsr(n, n + e, b.host.max_graph_edges + b.host.max_nodes, row_ptr.data_ptr(), col.data_ptr(), val.data_ptr())
-        b.lap = {"row_ptr": row_ptr, "col_idx": col, "values": val, "c": csr}
-        return b.lap
+        return {"row_ptr": row_ptr, "col_idx": col, "values": val, "c": csr, "faults": faults, "checked": False}
+
+    def _kept(self, made, status):
+        """A batch's kept supports for one more call.  "faults": the word their kernel wrote (None or absent: supports from elsewhere);
+        "checked": the host has read it and it is 0.  (The word stays with them: a captured call may read it again.)"""
+        if made.get("faults") is not None and not made["checked"]:
+            if status is not None:
+                status.bitwise_or_(made["faults"])
+            elif not self.torch.cuda.is_current_stream_capturing():
+                self.check_status(made["faults"])
+                made["checked"] = True
+        return made
+
+    def _call_status(self, b: DeviceBatch):
+        """A status word for one call on the batch, the faults of its supports in it; makes the supports if need be."""
+        t = self.torch
+        if b.lap is None:
+            b.lap = self._make_supports(b)
+        if b.lap.get("faults") is None or b.lap["checked"]:
+            return t.zeros(1, dtype=t.int32, device=self.device)
+        return b.lap["faults"] + 0
 
     def supports2(self, b: DeviceBatch, status=None):
         """T_2 = L.L for the batch, formed explicitly like the reference's ``t_k[-1]*laplacian``
-        (gcn/utils.py:268-271); float32 values bit-identical to the reference's.  Cached on the batch.
+        (gcn/utils.py:268-271); float32 values bit-identical to the reference's.  Kept with the batch, its faults too (``supports``).
         One device-to-host read of the entry count between the two passes (the caller allocates)."""
         t = self.torch
         if getattr(b, "lap2", None) is not None:
-            return b.lap2
+            return self._kept(b.lap2, status)
         n = b.host.num_nodes
-        own = status is None
-        if own:
-            status = t.zeros(1, dtype=t.int32, device=self.device)
+        faults = t.zeros(1, dtype=t.int32, device=self.device)
         tab = self._dinv(b.host.max_degree)
         row_ptr = t.zeros(n + 1, dtype=t.int32, device=self.device)
         _lib.check(self.lib.dgcn_supports2_count_batch(C.byref(b.c), tab.data_ptr(), int(tab.numel()), row_ptr.data_ptr(),
-                                                       status.data_ptr(), self._stream()), "dgcn_supports2_count_batch")
+                                                       faults.data_ptr(), self._stream()), "dgcn_supports2_count_batch")
         nnz = int(row_ptr[n].item())
         col = t.empty(max(nnz, 1), dtype=t.int32, device=self.device)
         val = t.empty(max(nnz, 1), dtype=t.float32, device=self.device)
         _lib.check(self.lib.dgcn_supports2_fill_batch(C.byref(b.c), tab.data_ptr(), int(tab.numel()), row_ptr.data_ptr(),
-                                                      col.data_ptr(), val.data_ptr(), status.data_ptr(), self._stream()),
+                                                      col.data_ptr(), val.data_ptr(), faults.data_ptr(), self._stream()),
                    "dgcn_supports2_fill_batch")
-        if own:
-            self.check_status(status)
+        if status is None:
+            self.check_status(faults)
         csr = _lib.DgcnCsr(n, nnz, 0, row_ptr.data_ptr(), col.data_ptr(), val.data_ptr())
-        b.lap2 = {"row_ptr": row_ptr, "col_idx": col, "values": val, "c": csr}
-        return b.lap2
+        b.lap2 = {"row_ptr": row_ptr, "col_idx": col, "values": val, "c": csr, "faults": faults, "checked": status is None}
+        return self._kept(b.lap2, status)
 
     # ------------------------------------------------------------------ K4
     def spmm(self, csr: dict, Z, C_feat: int, ldz: Optional[int] = None, graph_ptr=None, num_graphs=0, max_nodes=0,
@@ -453,8 +475,10 @@ class Engine:
     def forward(self, b: DeviceBatch, model: DeviceModel, X=None, x_const: Optional[float] = None,
                 mode: int = MODE_LAYERED, out=None):
         """scores[num_nodes, out_dim] (float32) = model.outputs for every node of the batch."""
+        return self._forward(b, self.supports(b), model, X, x_const, mode, out)
+
+    def _forward(self, b, lap, model, X, x_const, mode, out):
         t = self.torch
-        lap = self.supports(b)
         if x_const is None:
             x_const = float(np.float32(1.0 / model.in_dim))  # row-normalised all-ones features
         if out is None:
@@ -522,24 +546,34 @@ class Engine:
         """scores[num_nodes, out_dim] of a batch whose graph g belongs to model ``model_of_graph[g]`` (int32 on the device), layer by
         layer, one product and one aggregation launch each for the whole batch.  A float32 bank without biases returns the bits of
         ``forward`` with each graph's own model (biases are added before the neighbours' sum here and behind it there); an 8-bit bank is
-        an approximation whose error is the quantisation's.  ``status``: as in ``transform_grouped``."""
+        an approximation whose error is the quantisation's.  ``status``: as in ``transform_grouped``; the faults of the batch's
+        adjacency (``supports``) are reported by every call."""
+        scores, word = self._forward_bank(b, bank, model_of_graph, X, x_const, status)
+        if status is None and b.host.num_nodes:
+            self.check_status(word)
+            b.lap["checked"] = True
+        return scores
+
+    def _forward_bank(self, b, bank, model_of_graph, X, x_const, status):
+        """-> (scores, status word: the caller's, or one of this call with the faults of the batch's supports)."""
         t = self.torch
         B, n = b.host.num_graphs, b.host.num_nodes
         _array(model_of_graph, "model_of_graph", t.int32, (B,))
         if X is not None:
             _matrix(X, "X", (t.float32,), cols=bank.in_dim, rows=n)
         self._here(model_of_graph, X)
-        own = status is None
-        if own:
-            status = t.zeros(1, dtype=t.int32, device=self.device)
         if n == 0:
-            return t.empty((0, bank.out_dim), dtype=t.float32, device=self.device)
+            return (t.empty((0, bank.out_dim), dtype=t.float32, device=self.device),
+                    t.zeros(1, dtype=t.int32, device=self.device) if status is None else status)
         if x_const is None:
             x_const = float(np.float32(1.0 / bank.in_dim))
         if b.lap is None and t.cuda.is_current_stream_capturing():
             raise _lib.DgcnError("the batch's supports are made once and kept: call supports(b) before the capture")
         with t.cuda.device(self._index()):
-            lap = self.supports(b, status=status)
+            if status is None:
+                status, lap = self._call_status(b), b.lap
+            else:
+                lap = self.supports(b, status=status)
             H = X
             for l, lyr in enumerate(bank.layers):
                 out = lyr["out"]
@@ -552,9 +586,7 @@ class Engine:
                                                h_const=x_const, precise=l == 1, status=status)
                 H = self.spmm(lap, Z[:, out:], out, ldz=2 * out, graph_ptr=b.graph_ptr, num_graphs=B, max_nodes=b.host.max_nodes, Y0=Z,
                               ldy0=2 * out, act=lyr["act"], precise=l == 0)
-        if own:
-            self.check_status(status)
-        return H
+        return H, status
 
     def head_dual(self, b: DeviceBatch, act):
         """GCN2_DQN(is_dual=True) output head (gcn/models.py:651-653): [num_nodes, D] -> [num_nodes, D - 1]."""
@@ -649,13 +681,12 @@ class Engine:
             raise ValueError("batch has no vertex weights")
         if model.out_dim != 1:
             raise _lib.DgcnError("solve() needs a model with one output per node (diver_num=1)")
-        status = self.torch.zeros(1, dtype=self.torch.int32, device=self.device)
         if b.host.num_nodes == 0:
-            return self._empty_solution(b, status)
+            return self._empty_solution(b, self.torch.zeros(1, dtype=self.torch.int32, device=self.device))
         if mode == MODE_FUSED:
             return self.solve_fused(b, model, predict=predict, X=X, x_const=x_const)
-        self.supports(b, status=status)  # no host sync on the path: faults surface through res["status"]
-        scores = self.forward(b, model, X=X, x_const=x_const, mode=mode)
+        status = self._call_status(b)  # no host sync on the path: faults surface through res["status"]
+        scores = self._forward(b, b.lap, model, X, x_const, mode, None)
         res = self.lgs(b, scores=scores, weights=b.weights if predict == "mwis" else None, sum_weights=b.weights,
                        status=status)
         res["scores"] = scores
@@ -668,8 +699,7 @@ class Engine:
             raise ValueError("batch has no vertex weights")
         if bank.out_dim != 1:
             raise _lib.DgcnError("solve_bank() needs models with one output per node (diver_num=1)")
-        status = self.torch.zeros(1, dtype=self.torch.int32, device=self.device)
-        scores = self.forward_bank(b, bank, model_of_graph, X=X, x_const=x_const, status=status)
+        scores, status = self._forward_bank(b, bank, model_of_graph, X, x_const, None)
         if b.host.num_nodes == 0:
             return self._empty_solution(b, status)
         res = self.lgs(b, scores=scores, weights=b.weights if predict == "mwis" else None, sum_weights=b.weights, status=status)

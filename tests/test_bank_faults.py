@@ -1,0 +1,139 @@
+"""CPU: who learns that a batch's supports were made from a faulty adjacency - every call on the batch, not the first alone.
+
+The Engine's device calls are stood in for on the host: the supports launch writes its fault bits, everything else does nothing."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from distgcn_amd import _lib, datagen
+from distgcn_amd.batch import DeviceBatch, HostBatch
+from distgcn_amd.engine import DeviceModel, Engine
+
+SELF_LOOP = _lib.FAULT_SELF_LOOP
+
+
+class _Lib:
+    """The launches of Engine.supports / supports2 / forward / lgs; `faults` is what the supports kernels would find."""
+
+    def __init__(self, faults):
+        self.faults, self.made = faults, 0
+
+    def _word(self, address):
+        C.c_int32.from_address(address).value |= self.faults
+
+    def dgcn_supports_batch(self, b, tab, n, row, col, val, status, stream):
+        self.made += 1
+        self._word(status)
+        return 0
+
+    def dgcn_supports2_count_batch(self, b, tab, n, row, status, stream):
+        self._word(status)
+        return 0
+
+    def dgcn_supports2_fill_batch(self, b, tab, n, row, col, val, status, stream):
+        self.made += 1
+        self._word(status)
+        return 0
+
+    def dgcn_gcn_forward_workspace(self, *a):
+        return 256
+
+    def dgcn_gcn_forward_batch(self, *a):
+        return 0
+
+    def dgcn_lgs_batch(self, *a):
+        return 0
+
+    dgcn_transform_grouped_batch = None  # (never reached: the Engine's _launch is stood in for)
+
+
+@pytest.fixture()
+def host(monkeypatch):
+    import torch
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    e = Engine.__new__(Engine)
+    e.torch, e.device, e.lib, e._table, e._ws = torch, torch.device("cpu"), _Lib(0), None, None
+    e._codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    e._stream, e._index, e._here, e._launch = lambda: None, lambda: -1, lambda *a: None, lambda *a: None
+    hb = HostBatch(np.array([0, 2, 5]), np.array([0, 1, 2, 3, 5, 6]), np.array([1, 0, 3, 2, 4, 3]), np.ones(5))
+    e.batch = lambda: DeviceBatch(hb, e.device)
+    model = datagen.random_model(2, 4, seed=1)
+    e.bank, e.model, e.of = e.model_bank([model, model]), DeviceModel(model, "cpu"), torch.zeros(2, dtype=torch.int32)
+    e.spmm = lambda lap, Z, out, **kw: torch.zeros(5, out)
+    return e
+
+
+def test_forward_bank_raises_on_every_call(host):
+    host.lib.faults = SELF_LOOP
+    b = host.batch()
+    for _ in range(3):
+        with pytest.raises(_lib.DgcnError, match="self-loop"):
+            host.forward_bank(b, host.bank, host.of)
+    with pytest.raises(_lib.DgcnError, match="self-loop"):
+        host.forward(b, host.model)
+    with pytest.raises(_lib.DgcnError, match="self-loop"):
+        host.supports(b)
+
+
+def test_a_caller_s_word_gets_the_faults_every_time(host):
+    import torch
+    host.lib.faults = SELF_LOOP
+    b = host.batch()
+    for _ in range(3):
+        word = torch.zeros(1, dtype=torch.int32)
+        host.forward_bank(b, host.bank, host.of, status=word)
+        assert int(word) == SELF_LOOP
+        assert int(host.solve_bank(b, host.bank, host.of)["status"]) == SELF_LOOP
+        assert int(host.solve(b, host.model)["status"]) == SELF_LOOP
+    with pytest.raises(_lib.DgcnError, match="self-loop"):
+        host.forward_bank(b, host.bank, host.of)
+    with pytest.raises(_lib.DgcnError, match="self-loop"):
+        host.forward(b, host.model)
+
+
+def test_the_faults_are_the_batch_s_own(host):
+    """What else is in a caller's word does not become a fault of the batch, and a word the caller clears takes nothing back."""
+    import torch
+    b = host.batch()
+    word = torch.full((1,), _lib.FAULT_NAN_PRIORITY, dtype=torch.int32)
+    host.supports(b, status=word)
+    assert int(word) == _lib.FAULT_NAN_PRIORITY
+    res = host.solve(b, host.model)
+    res["status"].fill_(_lib.FAULT_NAN_PRIORITY)
+    assert int(host.solve(b, host.model)["status"]) == 0 and host.lib.made == 1
+    host.forward_bank(b, host.bank, host.of)
+    host.forward(b, host.model)
+    host.lib.faults = SELF_LOOP
+    bad = host.batch()
+    word.zero_()
+    host.supports(bad, status=word)
+    word.zero_()
+    assert int(host.solve(bad, host.model)["status"]) == SELF_LOOP
+    host.supports(b, status=word)
+    assert int(word) == 0
+    bad.lap = None  # made anew, by an adjacency without fault
+    host.lib.faults = 0
+    assert int(host.solve(bad, host.model)["status"]) == 0
+
+
+def test_second_supports_keep_their_faults(host):
+    import torch
+    host.lib.faults = _lib.FAULT_BAD_COLUMN
+    b = host.batch()
+    for _ in range(2):
+        word = torch.zeros(1, dtype=torch.int32)
+        host.supports2(b, status=word)
+        assert int(word) == _lib.FAULT_BAD_COLUMN
+    for _ in range(2):
+        with pytest.raises(_lib.DgcnError, match="column"):
+            host.supports2(b)
+
+
+def test_supports_from_elsewhere_have_no_faults(host):
+    b = host.batch()
+    host.supports(b)
+    b.lap = {k: v for k, v in b.lap.items() if k in ("row_ptr", "col_idx", "values", "c")}  # as a feed's own supports are set
+    assert int(host.solve(b, host.model)["status"]) == 0
+    host.forward(b, host.model)
+    host.forward_bank(b, host.bank, host.of)

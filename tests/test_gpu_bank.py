@@ -90,3 +90,65 @@ def test_greedy_search_stays_inside_its_graph(engine, sizes, degree, kw):
         assert int(state.max()) <= 2 and (kw.get("max_rounds") or int(state.min()) >= 1)
         if g in (0, 2):
             assert torch.equal(state, a["state"][lo:hi]) and int(a["rounds"][g]) == int(b["rounds"][g])
+
+
+def _self_loop_batch():
+    from distgcn_amd.batch import HostBatch
+    adjs, wts = _graphs([30, 50, 20], 2)
+    adjs[1] = adjs[1].tolil()
+    adjs[1][7, 7] = 1
+    adjs[1] = adjs[1].tocsr()
+    return HostBatch.from_scipy(adjs, wts)
+
+
+def test_a_faulty_batch_is_reported_by_every_call(engine):
+    import torch
+    from distgcn_amd import datagen
+    from distgcn_amd._lib import DgcnError
+    from distgcn_amd.engine import DeviceModel
+    hb = _self_loop_batch()
+    models = [datagen.random_model(3, 16, seed=s) for s in (1, 2)]
+    bank, dm = engine.model_bank(models), DeviceModel(models[0], "cuda:0")
+    mog = torch.tensor([0, 1, 1], dtype=torch.int32, device="cuda:0")
+    b = engine.upload(hb)
+    for _ in range(2):
+        with pytest.raises(DgcnError, match="self-loop"):
+            engine.forward_bank(b, bank, mog)
+    with pytest.raises(DgcnError, match="self-loop"):
+        engine.forward(b, dm)
+    b = engine.upload(hb)
+    for _ in range(2):
+        word = torch.zeros(1, dtype=torch.int32, device="cuda:0")
+        engine.forward_bank(b, bank, mog, status=word)
+        assert int(word) == 1 and int(engine.solve_bank(b, bank, mog)["status"]) == 1 and int(engine.solve(b, dm)["status"]) == 1
+    good = engine.upload(_batch_with_columns([30, 50, 20], 2, {})[0])
+    for _ in range(2):
+        assert int(engine.solve_bank(good, bank, mog)["status"]) == 0 and int(engine.solve(good, dm)["status"]) == 0
+        engine.forward_bank(good, bank, mog)
+
+
+def test_a_captured_pass_reports_its_batch_s_faults(engine):
+    import torch
+    from distgcn_amd import datagen
+    hb = _self_loop_batch()
+    bank = engine.model_bank([datagen.random_model(3, 16, seed=s) for s in (1, 2)])
+    mog = torch.tensor([0, 1, 1], dtype=torch.int32, device="cuda:0")
+    for host, want in ((hb, 1), (_batch_with_columns([30, 50, 20], 2, {})[0], 0)):
+        b, word = engine.upload(host), torch.zeros(1, dtype=torch.int32, device="cuda:0")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            engine.forward_bank(b, bank, mog, status=word)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = engine.forward_bank(b, bank, mog, status=word)
+        for _ in range(3):
+            word.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert int(word) == want
+            eager = torch.zeros(1, dtype=torch.int32, device="cuda:0")
+            assert torch.equal(out, engine.forward_bank(b, bank, mog, status=eager)) and int(eager) == want
+            if not want:
+                engine.forward_bank(b, bank, mog)  # (read on the host here: the word the graph reads stays)
