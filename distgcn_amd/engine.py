@@ -128,6 +128,25 @@ def _overlap(x, ldx, y, ldy):
     return pitch != ldy * ey or off < c * ex or off + d * ey > pitch
 
 
+def _apart(y, ldy, what, **arrays):
+    """Refuse contiguous tensors (None: not given) that share memory with a matrix; what lies between its rows is not part of it."""
+    rows, cols = y.shape
+    if not rows or not cols:
+        return
+    start, size = y.data_ptr(), y.element_size()
+    pitch, width = ldy * size, cols * size
+    for name, x in arrays.items():
+        if x is None:
+            continue
+        lo = x.data_ptr() - start
+        hi = lo + x.numel() * x.element_size()
+        if lo == hi or hi <= 0 or lo >= (rows - 1) * pitch + width:
+            continue
+        lo = max(lo, 0)
+        if lo % pitch < width or hi > (lo // pitch + 1) * pitch:
+            raise ValueError("%s shares memory with %s" % (what, name))
+
+
 def _array(x, what, dtype, shape):
     """Check a contiguous tensor of one dtype and shape."""
     if x.dtype != dtype:
@@ -405,6 +424,8 @@ class Engine:
             if _overlap(X, ldx, q, ldq):
                 raise ValueError("q shares memory with X")
             _array(scale, "scale", t.float32, (rows,))
+            _apart(X, ldx, "X", scale=scale)
+            _apart(q, ldq, "q", scale=scale)
         self._here(X, q, scale)
         self._launch(self.lib.dgcn_quantize_rows_batch, "dgcn_quantize_rows_batch", X.data_ptr(), codes[X.dtype], ldx, rows, cols,
                      q.data_ptr(), ldq, scale.data_ptr())
@@ -417,10 +438,13 @@ class Engine:
         t = self.torch
         if Wq.dtype != t.int8:
             raise TypeError("Wq is %s, expected torch.int8" % Wq.dtype)
+        given = out is not None
         rows, cin, ctot, _, ldh, code, dt, out, ldy = self._product_args(
             Hq, Wq, bias, act, dtype or (t.float32 if out is None else out.dtype), out, False)
         _array(h_scale, "h_scale", t.float32, (rows,))
         _array(w_scale, "w_scale", t.float32, (ctot,))
+        if given:
+            _apart(out, ldy, "out", h_scale=h_scale, w_scale=w_scale, bias=bias)
         self._here(Hq, Wq, h_scale, w_scale, bias, out)
         self._launch(self.lib.dgcn_transform_int8_batch, "dgcn_transform_int8_batch", Hq.data_ptr(), ldh, h_scale.data_ptr(), rows, cin,
                      Wq.data_ptr(), w_scale.data_ptr(), ctot, None if bias is None else bias.data_ptr(), code, out.data_ptr(), dt, ldy)
@@ -439,9 +463,12 @@ class Engine:
             raise ValueError("constant features need float32 weights and the number of rows")
         if precise and W.dtype != t.float32:
             raise ValueError("precise takes float32")
+        given = out is not None
         rows, cin, ctot, M, ldh, code, dt, out, ldy = self._product_args(H, W, bias, act, W.dtype, out, True, rows)
         self._here(H, W, bias, out)
         G, status, own = self._groups(group_ptr, model_of_group, M, status)
+        if given:
+            _apart(out, ldy, "out", bias=bias, group_ptr=group_ptr, model_of_group=model_of_group, status=status)
         self._launch(self.lib.dgcn_transform_grouped_batch, "dgcn_transform_grouped_batch", None if H is None else H.data_ptr(), dt, ldh,
                      float(h_const), rows, cin, group_ptr.data_ptr(), None if model_of_group is None else model_of_group.data_ptr(), G,
                      W.data_ptr(), M, ctot, None if bias is None else bias.data_ptr(), code, 1 if precise else 0, out.data_ptr(), ldy,
@@ -457,12 +484,15 @@ class Engine:
         t = self.torch
         if Wq.dtype != t.int8:
             raise TypeError("Wq is %s, expected torch.int8" % Wq.dtype)
+        given = out is not None
         rows, cin, ctot, M, ldh, code, dt, out, ldy = self._product_args(
             Hq, Wq, bias, act, dtype or (t.float32 if out is None else out.dtype), out, True)
         _array(h_scale, "h_scale", t.float32, (rows,))
         _array(w_scale, "w_scale", t.float32, (M, ctot))
         self._here(Hq, Wq, h_scale, w_scale, bias, out)
         G, status, own = self._groups(group_ptr, model_of_group, M, status)
+        if given:
+            _apart(out, ldy, "out", h_scale=h_scale, w_scale=w_scale, bias=bias, group_ptr=group_ptr, model_of_group=model_of_group, status=status)
         self._launch(self.lib.dgcn_transform_grouped_int8_batch, "dgcn_transform_grouped_int8_batch", Hq.data_ptr(), ldh,
                      h_scale.data_ptr(), rows, cin, group_ptr.data_ptr(), None if model_of_group is None else model_of_group.data_ptr(), G,
                      Wq.data_ptr(), w_scale.data_ptr(), M, ctot, None if bias is None else bias.data_ptr(), code, out.data_ptr(), dt, ldy,

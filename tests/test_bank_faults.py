@@ -137,3 +137,79 @@ def test_supports_from_elsewhere_have_no_faults(host):
     assert int(host.solve(b, host.model)["status"]) == 0
     host.forward(b, host.model)
     host.forward_bank(b, host.bank, host.of)
+
+
+@pytest.fixture()
+def checks():
+    """An Engine on the host whose argument checks run; a call that passes them all raises AssertionError("accepted")."""
+    import torch
+    e = Engine.__new__(Engine)
+    e.torch, e.device, e.lib = torch, torch.device("cpu"), _lib.load()
+    e._codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    e._here = lambda *a: None
+
+    def launched(*a):
+        raise AssertionError("accepted")
+    e._launch = launched
+    return e
+
+
+def _refused(call, **kw):
+    with pytest.raises(ValueError, match="shares memory"):
+        call(**kw)
+
+
+def _taken(call, **kw):
+    with pytest.raises(AssertionError, match="accepted"):
+        call(**kw)
+
+
+def test_outputs_apart_from_scales_biases_and_tables(checks):
+    import torch
+    e = checks
+    buf = torch.zeros(64 * 16)
+    at = lambda lo, *shape: buf[lo:lo + int(np.prod(shape))].view(*shape)
+    ints = lambda lo, n: at(lo, n).view(torch.int32)
+    out = at(256, 8, 16)[:, :10]  # elements 256 .. 383, six free ones behind each row's ten
+    H, W = torch.zeros(8, 4), torch.zeros(2, 10, 4)
+    h8, w8 = torch.zeros(8, 4, dtype=torch.int8), torch.zeros(2, 10, 4, dtype=torch.int8)
+    ptr, mog, word = torch.tensor([0, 3, 8], dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    hs, ws, bias = torch.zeros(8), torch.zeros(2, 10), torch.zeros(2, 10)
+    f = lambda **kw: e.transform_grouped(**{**dict(H=H, W=W, group_ptr=ptr, model_of_group=mog, bias=bias, out=out, status=word), **kw})
+    g = lambda **kw: e.transform_grouped_int8(**{**dict(Hq=h8, h_scale=hs, Wq=w8, w_scale=ws, group_ptr=ptr, model_of_group=mog, bias=bias, out=out, status=word), **kw})
+    d = lambda **kw: e.transform_int8(**{**dict(Hq=h8, h_scale=hs, Wq=w8[0], w_scale=ws[0], bias=bias[0], out=out), **kw})
+    for call in (f, g):
+        _taken(call)
+        for lo in (256 - 19, 256, 262, 266, 276, 383 - 16 - 6):  # into the first row, over it, from a gap into the next row, the last row
+            _refused(call, bias=at(lo, 2, 10))
+        _taken(call, bias=at(256 - 20, 2, 10))
+        _taken(call, bias=at(378, 2, 10))  # behind the last row's ten
+        _refused(call, group_ptr=ints(256 + 32 + 8, 3))
+        _taken(call, group_ptr=ints(256 + 32 + 10, 3))  # a gap
+        _refused(call, group_ptr=ints(256 + 32 + 14, 3))
+        _refused(call, model_of_group=ints(256 + 9, 2))
+        _refused(call, status=ints(256 + 48, 1))
+        _taken(call, status=ints(256 + 48 - 1, 1))
+    _taken(g, h_scale=at(0, 8), w_scale=at(8, 2, 10))
+    _refused(g, h_scale=at(250, 8))
+    _refused(g, w_scale=at(370, 2, 10))
+    _taken(d)
+    _refused(d, h_scale=at(250, 8))
+    _refused(d, w_scale=at(250, 10))
+    _refused(d, bias=at(270, 10))
+    X, q = at(256, 8, 16)[:, :10], at(512, 8, 16).view(torch.int8)[:, :10]
+    qz = lambda scale: e.quantize_rows(X, out=(q, scale))
+    _taken(qz, scale=at(0, 8))
+    _taken(qz, scale=at(512 - 8, 8))
+    for lo in (250, 300, 376, 505, 512, 521):
+        _refused(qz, scale=at(lo, 8))
+    _taken(qz, scale=at(512 + 16 * 3 + 3, 8))  # q's rows take 10 bytes of 64
+
+
+def test_empty_outputs_share_nothing(checks):
+    import torch
+    e, z = checks, torch.zeros
+    buf = z(100)
+    _taken(e.transform_grouped, H=z(0, 4), W=z(1, 10, 4), group_ptr=torch.zeros(2, dtype=torch.int32), bias=buf[:10].view(1, 10), out=buf[:0].view(0, 10),
+           status=torch.zeros(1, dtype=torch.int32))
+    _taken(e.quantize_rows, X=z(0, 4), out=(z(0, 4, dtype=torch.int8), z(0)))
