@@ -3,14 +3,16 @@
 # Not part of the product: built on demand (here or on the GPU box: hipcc cross-compiles), selected with
 # DGCN_LIB=distgcn_amd/libdgcn_diag.so.  One object per source, side by side, like __graft_entry__.build().
 set -e
-cd "$(dirname "$0")/../distgcn_amd/csrc"
-mkdir -p ../../build/obj_diag
-SRCS="runtime pack supports supports2 spmm transform layer forward lgs fused shallow expand host_solver general big tail wide big2"
+. "$(dirname "$0")/library_build.sh"
+cd "$ROOT/distgcn_amd/csrc"
+OBJ="$ROOT/build/obj_diag"
+mkdir -p "$OBJ"
 for s in $SRCS; do
-  if [ ! -f ../../build/obj_diag/$s.o ] || [ -n "$(find $s.hip *.h ../../include/dgcn.h -newer ../../build/obj_diag/$s.o 2>/dev/null | head -1)" ]; then
-    hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -DDGCN_DIAG -c $s.hip -o ../../build/obj_diag/$s.o &
+  if [ ! -f "$OBJ/$s.o" ] || [ -n "$(find $s.hip *.h ../../include/dgcn.h ../../__graft_entry__.py -newer "$OBJ/$s.o" 2>/dev/null | head -1)" ]; then
+    rm -f "$OBJ/$s.o"  # (a source that does not compile must not leave its old object to the link)
+    "$HIPCC" $FLAGS -DDGCN_DIAG -c $s.hip -o "$OBJ/$s.o" &
   fi
 done
 wait
-OBJS=""; for s in $SRCS; do OBJS="$OBJS ../../build/obj_diag/$s.o"; done
-hipcc --offload-arch=gfx950 -fPIC -shared -Wl,-z,defs -o ../libdgcn_diag.so $OBJS
+OBJS=""; for s in $SRCS; do OBJS="$OBJS $OBJ/$s.o"; done
+"$HIPCC" $FLAGS -shared -Wl,-z,defs -o ../libdgcn_diag.so $OBJS

@@ -1,6 +1,7 @@
 #!/bin/bash
 # Register / spill / scratch summary of every kernel in one source file: tools/resusage.sh fused.hip [extra flags]
-cd "$(dirname "$0")/../distgcn_amd/csrc" && hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -c "$1" -o /tmp/resusage.o "${@:2}" \
+. "$(dirname "$0")/library_build.sh"
+cd "$ROOT/distgcn_amd/csrc" && "$HIPCC" $FLAGS -c "$1" -o /tmp/resusage.o "${@:2}" \
   -Rpass-analysis=kernel-resource-usage 2>&1 | awk '
   /Function Name:/ {name=$0; sub(/.*Function Name: /,"",name); sub(/ \[.*/,"",name)}
   /    VGPRs:/ {v=$0; sub(/.*VGPRs: /,"",v); sub(/ \[.*/,"",v)}
