@@ -14,7 +14,7 @@ LIB_PATH = os.environ.get("DGCN_LIB") or os.path.join(_HERE, "libdgcn.so")
 
 OK = 0
 ACT_LINEAR, ACT_LEAKY_RELU, ACT_RELU = 0, 1, 2
-F32, BF16, F16 = 0, 1, 2  # DGCN_F32 / DGCN_BF16 / DGCN_F16
+F32, BF16, F16, I8 = 0, 1, 2, 3  # DGCN_F32 / DGCN_BF16 / DGCN_F16 / DGCN_I8 (dgcn_product_path only)
 FAULT_SELF_LOOP, FAULT_NAN_PRIORITY, FAULT_DEGREE_RANGE, FAULT_BAD_COLUMN = 1, 2, 4, 8
 FAULT_NAMES = {
     FAULT_SELF_LOOP: "adjacency has a self-loop (heuristics.py:94 would never terminate)",
@@ -28,7 +28,7 @@ FAULT_NAMES = {
 # every symbol include/dgcn.h declares; tests/test_cabi.py checks the library exports them all
 SYMBOLS = (
     "dgcn_version", "dgcn_last_error", "dgcn_pack_measure", "dgcn_pack_batch", "dgcn_pack_compact_layout", "dgcn_pack_compact_batch", "dgcn_expand_compact_batch", "dgcn_supports_batch", "dgcn_supports2_count_batch", "dgcn_supports2_fill_batch", "dgcn_spmm_split", "dgcn_set_cluster", "dgcn_get_cluster", "dgcn_spmm_batch", "dgcn_spmm_f64acc_batch", "dgcn_transform_batch", "dgcn_transform_f64acc_batch",
-    "dgcn_quantize_rows_batch", "dgcn_transform_int8_batch", "dgcn_transform_grouped_batch", "dgcn_transform_grouped_int8_batch",
+    "dgcn_quantize_rows_batch", "dgcn_transform_int8_batch", "dgcn_transform_grouped_batch", "dgcn_transform_grouped_int8_batch", "dgcn_product_path",
     "dgcn_gcn_forward_workspace", "dgcn_gcn_forward_batch", "dgcn_gcn_forward_poly_batch", "dgcn_head_dual_batch", "dgcn_head_skip_batch", "dgcn_argmax_batch", "dgcn_lgs_batch", "dgcn_margin_risk_batch", "dgcn_lgs_masked_batch", "dgcn_solve_supported", "dgcn_solve_path", "dgcn_set_general", "dgcn_get_general", "dgcn_solve_workspace", "dgcn_solve_batch", "dgcn_solve_residual_batch",
     "dgcn_host_solver_create", "dgcn_host_solver_destroy", "dgcn_host_solver_submit", "dgcn_host_solver_result",
     "dgcn_timing_enable", "dgcn_timing_reset", "dgcn_timing_read", "dgcn_timing_sampling",
@@ -139,6 +139,8 @@ def load():
     lib.dgcn_transform_grouped_batch.argtypes = [vp, i32, i64, f32, i32, i32, vp, vp, i32, vp, i32, i32, vp, i32, i32, vp, i64, vp, vp]
     lib.dgcn_transform_grouped_int8_batch.restype = C.c_int
     lib.dgcn_transform_grouped_int8_batch.argtypes = [vp, i64, vp, i32, i32, vp, vp, i32, vp, vp, i32, i32, vp, i32, vp, i32, i64, vp, vp]
+    lib.dgcn_product_path.restype = C.c_int
+    lib.dgcn_product_path.argtypes = [i32, i32, vp, i64, i32, i32, i32, vp, i32, vp, i32, i64]
     lib.dgcn_gcn_forward_workspace.restype = sz
     lib.dgcn_gcn_forward_workspace.argtypes = [C.POINTER(DgcnBatch), C.POINTER(DgcnModel), i32]
     lib.dgcn_gcn_forward_batch.restype = C.c_int

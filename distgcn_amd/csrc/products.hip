@@ -862,6 +862,14 @@ template <int KIND, int TN, int KS> static int launch_rows(const char* family, c
     else return launch_rows_as<KIND, _Float16, TN, KS>(family, a, s);
 }
 
+// What a call launches: kernels by number, tile kernels with DIRECT.
+enum Path {
+    P_64_64, P_128_128, P_128_256, P_192_256, P_256_256,  // k_product, 8- and 16-bit types' shapes (in kDirect's order); P_64_64 and P_128_128 float32 too
+    P_128_16, P_128_32, P_32_64,                          // k_product, float32
+    P_FEW_2_4, P_FEW_1_8, P_FEW_1_4,                      // k_product_few<NT, WAVES>
+    P_ROWS_16, P_ROWS_32,                                 // k_product_rows, up to 16 / 32 columns
+};
+
 // The tile shapes of the 8- and 16-bit products and what they cost, fitted to 26 shapes of 128 .. 100 000 rows, k of 64 .. 4 096 bytes and
 // 20 .. 4 096 columns, dense and in 8 .. 300 groups: a stage (128 bytes of k) takes s1 us in a workgroup that has its CU to itself and sc
 // us with per_cu of them there, a tile's start and end f us.  The least estimate is the fastest shape or within 14 % of it on 22 of the
@@ -917,61 +925,88 @@ static int choose_shape(ProductArgs& a, int64_t row_bytes, bool direct) {
     return best;
 }
 
-template <int KIND> static int dispatch_kind(const char* family, ProductArgs& a, hipStream_t s) {
+// The kernel of a call; sets a.stream.
+template <int KIND> static int choose_path(ProductArgs& a) {
     const int64_t row_bytes = (int64_t)a.cin * Elem<KIND>::size;
     if constexpr (KIND == K_F32P) {
-        return launch_tiles<KIND, 64, 64, 2, 2, 2>(family, a, s);
+        return P_64_64;
     } else {
         // a narrow layer over very many rows: no tile would be more than a copy (800 000 rows of 32 float32 -> 2: 28 us against 32 of the
         // 128 x 16 tile; 300 000 rows of 32 bf16 -> 32: 12 against 19 of 64 x 64; at 60 000 rows no difference)
         if (a.H && a.dwords_h && a.dwords_w && row_bytes % 16 == 0 && row_bytes <= 128 && a.ctot <= 32 && a.rows >= 1 << 17)
-            return a.ctot <= 16 ? launch_rows<KIND, 1, 2>(family, a, s) : launch_rows<KIND, 2, 2>(family, a, s);
+            return a.ctot <= 16 ? P_ROWS_16 : P_ROWS_32;
     }
     const int groups = min(a.num_groups, a.rows);
-    if constexpr (KIND == K_F32) a.stream = streams_out(a, row_bytes, (float)a.rows * a.ctot * a.cin * 2.f / 149e6f);
     if constexpr (KIND == K_F32) {
+        a.stream = streams_out(a, row_bytes, (float)a.rows * a.ctot * a.cin * 2.f / 149e6f);
         // float32: the matrix pipe is the bound from some 64 columns on, so the shape matters little but for its waste.  128 x 128 (1 024
         // x 1 024, 8 192 rows: 144 us against 165) where its tiles fill whole rounds of two per CU; 64 x 64 where a row is one stage (32
         // -> 64, 500 graphs: 16.4 against 19.4 of 32 x 64), else 32 x 64 (128 -> 256: 96 against 101; 200 rows in 10 groups: 12 against 15).
         const float rounds = expected_slots(a, 128) * (float)((a.ctot + 127) / 128) / (2 * kCUs);
-        if (a.ctot <= 16) return launch_tiles<KIND, 128, 16, 4, 1, 2>(family, a, s);
-        if (a.ctot <= 32 && row_bytes > 128) return launch_tiles<KIND, 128, 32, 4, 1, 2>(family, a, s);
-        if (groups == 1 && row_bytes >= 1024 && rounds > .9f * ceilf(rounds)) return launch_tiles<KIND, 128, 128, 2, 4, 2>(family, a, s);
-        if (row_bytes <= 128 && a.rows / groups >= 48) return launch_tiles<KIND, 64, 64, 2, 2, 2>(family, a, s);
-        return launch_tiles<KIND, 32, 64, 1, 4, 2>(family, a, s);
+        if (a.ctot <= 16) return P_128_16;
+        if (a.ctot <= 32 && row_bytes > 128) return P_128_32;
+        if (groups == 1 && row_bytes >= 1024 && rounds > .9f * ceilf(rounds)) return P_128_128;
+        return row_bytes <= 128 && a.rows / groups >= 48 ? P_64_64 : P_32_64;
     } else if constexpr (KIND != K_F32P) {
         // few rows in every group, long rows and not enough tiles to fill the chip: split k over a workgroup's waves (1 row, 4 096 x
         // 4 096 int8: 6 us against 17 of the 64 x 64 tile; 64 rows: 15 against 19; 24 rows in 64 groups, fp16 2 048 x 1 024: 23 against 29)
         const int64_t tiles = (a.gptr ? (int64_t)groups : (a.rows + 63) / 64) * ((a.ctot + 63) / 64);
         if (row_bytes >= 512 && a.rows <= (a.gptr ? 16 * (int64_t)groups : 64) && tiles < 2 * kCUs) {
-            if (a.gptr || a.rows > 16) return launch_few<KIND, 2, 4>(family, a, s);
-            return row_bytes >= 2048 ? launch_few<KIND, 1, 8>(family, a, s) : launch_few<KIND, 1, 4>(family, a, s);
+            if (a.gptr || a.rows > 16) return P_FEW_2_4;
+            return row_bytes >= 2048 ? P_FEW_1_8 : P_FEW_1_4;
         }
-        const bool direct = direct_loads<KIND>(a);
-        switch (choose_shape(a, row_bytes, direct)) {
-            case 0: return launch_tiles<KIND, 64, 64, 2, 2, 2>(family, a, s);
-            case 1: return launch_tiles<KIND, 128, 128, 2, 4, 2>(family, a, s);
-            case 2: return launch_tiles<KIND, 128, 256, 2, 4, 3>(family, a, s);
-            case 3: return launch_tiles<KIND, 192, 256, 2, 4, 2>(family, a, s);
-            default: return launch_tiles_as<KIND, 256, 256, 2, 4, 2, true>(family, a, s);
+        return choose_shape(a, row_bytes, direct_loads<KIND>(a));
+    }
+}
+
+template <int KIND> static int launch_path(int path, const char* family, const ProductArgs& a, hipStream_t s) {
+    if constexpr (KIND == K_F32P) {
+        return launch_tiles<KIND, 64, 64, 2, 2, 2>(family, a, s);
+    } else {
+        if (path == P_ROWS_16) return launch_rows<KIND, 1, 2>(family, a, s);
+        if (path == P_ROWS_32) return launch_rows<KIND, 2, 2>(family, a, s);
+        if (path == P_64_64) return launch_tiles<KIND, 64, 64, 2, 2, 2>(family, a, s);
+        if (path == P_128_128) return launch_tiles<KIND, 128, 128, 2, 4, 2>(family, a, s);
+        if constexpr (KIND == K_F32) {
+            if (path == P_128_16) return launch_tiles<KIND, 128, 16, 4, 1, 2>(family, a, s);
+            if (path == P_128_32) return launch_tiles<KIND, 128, 32, 4, 1, 2>(family, a, s);
+            return launch_tiles<KIND, 32, 64, 1, 4, 2>(family, a, s);
+        } else {
+            if (path == P_FEW_2_4) return launch_few<KIND, 2, 4>(family, a, s);
+            if (path == P_FEW_1_8) return launch_few<KIND, 1, 8>(family, a, s);
+            if (path == P_FEW_1_4) return launch_few<KIND, 1, 4>(family, a, s);
+            if (path == P_128_256) return launch_tiles<KIND, 128, 256, 2, 4, 3>(family, a, s);
+            if (path == P_192_256) return launch_tiles<KIND, 192, 256, 2, 4, 2>(family, a, s);
+            return launch_tiles_as<KIND, 256, 256, 2, 4, 2, true>(family, a, s);
         }
     }
 }
 
-static int product_dispatch(const char* family, int kind, ProductArgs& a, hipStream_t s) {
+static void prepare_args(int kind, ProductArgs& a) {
     const int es = kind == K_I8 ? 1 : kind == K_BF16 || kind == K_F16 ? 2 : 4;
     // Counting pays where a tile is long (16 000 rows of 1 024 bytes in 64 groups, 512 columns, int8: 20 us, searching 31; of 4 096 bytes 58
     // against 91); in short ones its loads are a part of the time (40 000 rows of 128 bytes in 8 groups: 20 against 17; in 250: 29 against 25).
     a.counted = a.gptr && a.num_groups <= kCountedGroups && (int64_t)a.cin * es > 256;
     a.dwords_h = (uintptr_t)a.H % 4 == 0 && a.ldh * es % 4 == 0;
     a.dwords_w = (uintptr_t)a.W % 4 == 0 && (int64_t)a.cin * es % 4 == 0;
+}
+
+template <class F> static int with_kind(int kind, F f) {
     switch (kind) {
-        case K_I8: return dispatch_kind<K_I8>(family, a, s);
-        case K_BF16: return dispatch_kind<K_BF16>(family, a, s);
-        case K_F16: return dispatch_kind<K_F16>(family, a, s);
-        case K_F32: return dispatch_kind<K_F32>(family, a, s);
-        default: return dispatch_kind<K_F32P>(family, a, s);
+        case K_I8: return f(std::integral_constant<int, K_I8>{});
+        case K_BF16: return f(std::integral_constant<int, K_BF16>{});
+        case K_F16: return f(std::integral_constant<int, K_F16>{});
+        case K_F32: return f(std::integral_constant<int, K_F32>{});
+        default: return f(std::integral_constant<int, K_F32P>{});
     }
+}
+
+static int product_dispatch(const char* family, int kind, ProductArgs& a, hipStream_t s) {
+    prepare_args(kind, a);
+    return with_kind(kind, [&](auto k) {
+        constexpr int KIND = decltype(k)::value;
+        return launch_path<KIND>(choose_path<KIND>(a), family, a, s);
+    });
 }
 
 static bool known_dtype(int32_t d) { return d == DGCN_F32 || d == DGCN_BF16 || d == DGCN_F16; }
@@ -1042,4 +1077,26 @@ extern "C" int dgcn_transform_grouped_batch(const void* H, int32_t dtype, int64_
     a.gptr = group_ptr; a.mog = model_of_group; a.status = status;
     const int kind = dtype == DGCN_BF16 ? K_BF16 : dtype == DGCN_F16 ? K_F16 : precise ? K_F32P : K_F32;
     return product_dispatch("transform_grouped", kind, a, (hipStream_t)stream);
+}
+
+extern "C" int dgcn_product_path(int32_t dtype, int32_t precise, const void* H, int64_t ldh, int32_t rows, int32_t cin, int32_t num_groups,
+                                 const void* W, int32_t ctot, const void* Y, int32_t out_dtype, int64_t ldy) {
+    static const int32_t table = 0;  // (stands for a group table: nothing reads it)
+    const char* who = "dgcn_product_path";
+    const bool i8 = dtype == DGCN_I8;
+    int rc = check_sizes(who, rows, cin, ctot, i8 ? 1 : dtype == DGCN_F32 ? 4 : 2, H != nullptr, ldh, ldy, DGCN_ACT_LINEAR);
+    if (rc) return rc;
+    if ((!i8 && !known_dtype(dtype)) || !known_dtype(out_dtype)) return fail(DGCN_ERR_ARG, "%s: unknown dtype %d -> %d", who, dtype, out_dtype);
+    if (rows == 0 || num_groups < 0 || !W || !Y || (!H && dtype != DGCN_F32)) return fail(DGCN_ERR_ARG, "%s: no such product", who);
+    if (i8 ? precise : out_dtype != dtype || num_groups == 0 || (precise && dtype != DGCN_F32)) return fail(DGCN_ERR_ARG, "%s: no such product", who);
+    ProductArgs a{};
+    a.H = (const char*)H; a.ldh = ldh; a.rows = rows; a.cin = cin; a.W = (const char*)W; a.ctot = ctot; a.Y = const_cast<void*>(Y);
+    a.out_dtype = out_dtype; a.ldy = ldy; a.num_groups = num_groups > 0 ? num_groups : 1; a.gptr = num_groups > 0 ? &table : nullptr;
+    const int kind = i8 ? K_I8 : dtype == DGCN_BF16 ? K_BF16 : dtype == DGCN_F16 ? K_F16 : precise ? K_F32P : K_F32;
+    prepare_args(kind, a);
+    return with_kind(kind, [&](auto k) {
+        constexpr int KIND = decltype(k)::value;
+        const int path = choose_path<KIND>(a);
+        return path | (path < P_FEW_2_4 && direct_loads<KIND>(a) ? DGCN_PRODUCT_DIRECT : 0) | (a.stream ? DGCN_PRODUCT_STREAMS : 0);
+    });
 }

@@ -38,7 +38,7 @@ enum { DGCN_OK = 0, DGCN_ERR_ARG = -1, DGCN_ERR_LAUNCH = -2, DGCN_ERR_UNSUPPORTE
 enum { DGCN_ACT_LINEAR = 0, DGCN_ACT_LEAKY_RELU = 1, DGCN_ACT_RELU = 2 };
 
 /* element types of the entry points that take more than float32 */
-enum { DGCN_F32 = 0, DGCN_BF16 = 1, DGCN_F16 = 2 };
+enum { DGCN_F32 = 0, DGCN_BF16 = 1, DGCN_F16 = 2, DGCN_I8 = 3 /* dgcn_product_path only */ };
 
 /* bits OR-ed into *status by kernels */
 enum {
@@ -269,6 +269,14 @@ int dgcn_transform_grouped_int8_batch(const int8_t* H, int64_t ldh, const float*
                                       const int8_t* W, const float* w_scale, int32_t num_models, int32_t ctot,
                                       const float* bias, int32_t act, void* Y, int32_t out_dtype, int64_t ldy,
                                       int32_t* status, void* stream);
+/* Which kernel such a call launches (no launch happens; pointers are looked at for their alignment and for NULL only).  dtype: of H and W,
+ * DGCN_I8 for the 8-bit products; num_groups 0: dgcn_transform_int8_batch.  -> the kernel's number - tiles of 0: 64 x 64, 1: 128 x 128,
+ * 2: 128 x 256, 3: 192 x 256, 4: 256 x 256, 5: 128 x 16, 6: 128 x 32, 7: 32 x 64 rows x columns; few rows, 8: 32 columns and four waves,
+ * 9: 16 and eight, 10: 16 and four; many rows of at most 11: 16, 12: 32 columns - OR-ed with DGCN_PRODUCT_DIRECT (a tile loaded straight to
+ * LDS) and DGCN_PRODUCT_STREAMS (Y may be stored past the caches); < 0: a refused call. */
+enum { DGCN_PRODUCT_DIRECT = 16, DGCN_PRODUCT_STREAMS = 32 };
+int dgcn_product_path(int32_t dtype, int32_t precise, const void* H, int64_t ldh, int32_t rows, int32_t cin, int32_t num_groups,
+                      const void* W, int32_t ctot, const void* Y, int32_t out_dtype, int64_t ldy);
 
 /* ---- A4-A6: sess.run(model.outputs_softmax) for a batch (mwis_dqn_call.py:140-143) ------------
  * Precision (part of the ABI, mirrored by oracle/dgcn_oracle.c, identical in every mode and entry point): float32
