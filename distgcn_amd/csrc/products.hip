@@ -656,7 +656,9 @@ __global__ __launch_bounds__(WAVES * 64) void k_product_few(ProductArgs a, int s
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = (float)sum[i];
         const float hs = KIND == K_I8 ? a.hs[r] : 0.f;
-        if (a.out_dtype == DGCN_BF16) finish<KIND, __bf16, 4>(a, r, n, v, hs, ws, bias);
+        if constexpr (KIND == K_BF16) finish<KIND, __bf16, 4>(a, r, n, v, hs, ws, bias);
+        else if constexpr (KIND == K_F16) finish<KIND, _Float16, 4>(a, r, n, v, hs, ws, bias);
+        else if (a.out_dtype == DGCN_BF16) finish<KIND, __bf16, 4>(a, r, n, v, hs, ws, bias);
         else if (a.out_dtype == DGCN_F16) finish<KIND, _Float16, 4>(a, r, n, v, hs, ws, bias);
         else finish<KIND, float, 4>(a, r, n, v, hs, ws, bias);
     }
@@ -952,8 +954,9 @@ template <int KIND> static int choose_path(ProductArgs& a) {
         // 4 096 int8: 6 us against 17 of the 64 x 64 tile; 64 rows: 15 against 19; 24 rows in 64 groups, fp16 2 048 x 1 024: 23 against 29)
         const int64_t tiles = (a.gptr ? (int64_t)groups : (a.rows + 63) / 64) * ((a.ctot + 63) / 64);
         if (row_bytes >= 512 && a.rows <= (a.gptr ? 16 * (int64_t)groups : 64) && tiles < 2 * kCUs) {
-            if (a.gptr || a.rows > 16) return P_FEW_2_4;
-            return row_bytes >= 2048 ? P_FEW_1_8 : P_FEW_1_4;
+            if constexpr (KIND == K_I8)  // (the other types' entry point is the grouped one)
+                if (!a.gptr && a.rows <= 16) return row_bytes >= 2048 ? P_FEW_1_8 : P_FEW_1_4;
+            return P_FEW_2_4;
         }
         return choose_shape(a, row_bytes, direct_loads<KIND>(a));
     }
@@ -973,8 +976,10 @@ template <int KIND> static int launch_path(int path, const char* family, const P
             return launch_tiles<KIND, 32, 64, 1, 4, 2>(family, a, s);
         } else {
             if (path == P_FEW_2_4) return launch_few<KIND, 2, 4>(family, a, s);
-            if (path == P_FEW_1_8) return launch_few<KIND, 1, 8>(family, a, s);
-            if (path == P_FEW_1_4) return launch_few<KIND, 1, 4>(family, a, s);
+            if constexpr (KIND == K_I8) {
+                if (path == P_FEW_1_8) return launch_few<KIND, 1, 8>(family, a, s);
+                if (path == P_FEW_1_4) return launch_few<KIND, 1, 4>(family, a, s);
+            }
             if (path == P_128_256) return launch_tiles<KIND, 128, 256, 2, 4, 3>(family, a, s);
             if (path == P_192_256) return launch_tiles<KIND, 192, 256, 2, 4, 2>(family, a, s);
             return launch_tiles_as<KIND, 256, 256, 2, 4, 2, true>(family, a, s);

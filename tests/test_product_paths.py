@@ -1,6 +1,10 @@
 """CPU: the calls of test_gpu_product_paths.py reach every kernel of the dense products, each tile shape with both loaders.
 
 ``dgcn_product_path`` chooses as a launch does; a change of the sizes it chooses by shows here as a kernel that nothing tests."""
+import re
+import shutil
+import subprocess
+
 import pytest
 
 from distgcn_amd import _lib
@@ -72,6 +76,16 @@ def test_every_kernel_is_reached_by_a_test():
     for name, how in seen.items():
         if name.startswith("k_product<0,"):  # one kernel for the three output types
             assert {out for out, _, _ in how} == set(TYPES), name
+
+
+@pytest.mark.skipif(shutil.which("nm") is None, reason="no nm")
+def test_no_kernel_is_compiled_that_no_call_reaches():
+    symbols = subprocess.run(["nm", "-D", "--defined-only", _lib.LIB_PATH], capture_output=True, text=True, check=True).stdout
+    word = {"f": "float", "DF16b": "__bf16", "DF16_": "_Float16", "Lb0E": "false", "Lb1E": "true"}
+    compiled = set()
+    for name, args in re.findall(r"_ZN4dgcn\d+(k_product(?:_few|_rows)?)I((?:Li\d+E|Lb[01]E|DF16[b_]|f)+)EEv", symbols):
+        compiled.add("%s<%s>" % (name, ", ".join(word.get(x) or x[2:-1] for x in re.findall(r"Li\d+E|Lb[01]E|DF16[b_]|f", args))))
+    assert compiled and compiled - set(_reached()) == set() and set(_reached()) - compiled == set()
 
 
 @pytest.mark.parametrize("kw,text", [(dict(dtype=9), "unknown dtype"), (dict(dtype=_lib.I8, precise=1), "no such"), (dict(rows=0), "no such"), (dict(out=_lib.F16), "no such"),
