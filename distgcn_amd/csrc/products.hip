@@ -915,7 +915,7 @@ static int choose_shape(ProductArgs& a, int64_t row_bytes, bool direct) {
         const float per = expected_slots(a, p.bm) * (float)((a.ctot + p.bn - 1) / p.bn) / kCUs;  // tiles per CU
         const float rounds = floorf(per / p.per_cu), rest = per - rounds * p.per_cu;
         float cost = rounds * (p.sc * steps + p.f);
-        if (rest > .02f) cost += (p.s1 + (p.per_cu > 1 ? (p.sc - p.s1) * (ceilf(rest) - 1.f) / (p.per_cu - 1) : 0.f)) * steps + p.f;
+        if (rest > .02f || rounds == 0.f) cost += (p.s1 + (p.per_cu > 1 ? (p.sc - p.s1) * (ceilf(rest) - 1.f) / (p.per_cu - 1) : 0.f)) * steps + p.f;
         if (cost < least) { least = cost; best = i; }
     }
     // Where the bytes alone take longer than that, a copy's many small workgroups are best (100 000 rows, int8 127 -> 256: 33 us with 64 x 64

@@ -88,6 +88,14 @@ def test_no_kernel_is_compiled_that_no_call_reaches():
     assert compiled and compiled - set(_reached()) == set() and set(_reached()) - compiled == set()
 
 
+@pytest.mark.parametrize("kind", ["int8", "bfloat16", "float16"])
+def test_a_call_of_few_tiles_costs_one_at_least(kind):
+    """Up to five tiles of the largest shapes used to cost nothing, and the first free one won."""
+    for rows, cin, ctot, groups in [(1, 64, 64, 1), (16, 64, 64, 8), (100, 128, 200, 3), (154, 32, 64, 4), (130, 64, 128, 1), (100, 256, 200, 5)]:
+        assert _path(kind, rows, cin, ctot, groups, "float32" if kind == "int8" else kind) == 16
+    assert _path("int8", 100, 4096, 200, 0, "float32") == 16
+
+
 @pytest.mark.parametrize("kw,text", [(dict(dtype=9), "unknown dtype"), (dict(dtype=_lib.I8, precise=1), "no such"), (dict(rows=0), "no such"), (dict(out=_lib.F16), "no such"),
                                      (dict(groups=0), "no such"), (dict(dtype=_lib.BF16, out=_lib.BF16, H=None), "no such"), (dict(ldh=3), "bad sizes"),
                                      (dict(cin=0), "bad sizes"), (dict(rows=2 ** 31 - 1), "more than")])
