@@ -896,12 +896,15 @@ static float out_bytes(const ProductArgs& a) { return (float)a.rows * (a.out_dty
 
 // A call that takes about as long as its bytes do (`compute_us`: without them) and whose bytes are mostly Y stores it past the caches, in
 // whole 64-byte sectors (rows of 4 000 bytes, which are not, take twice as long that way): 100 000 rows, int8 128 -> 256 float32 24 us
-// against 40 with outputs that the caches do not already hold; the six layers of a 128-wide 8-bit bank over 500 graphs 565 us against
-// 615, aggregations included.  Calls that compute for longer lose by it (fp32 128 -> 256: 1 %).
+// against 40 with outputs that the caches do not already hold; the six layers of a 128-wide 8-bit bank over 500 graphs 571 us against
+// 588, aggregations included.  Calls that compute for longer lose by it (fp32 128 -> 256: 1 %), and a small Y is better left in the caches for
+// the call that reads it (six layers of a float32 bank, aggregations included: 72.4 us against 75.7 with 1.0 MB per layer, 81.0 against
+// 81.6 with 2.6; 97.2 against 95.0 with 5.1, 178 against 170 with 20).
+constexpr float kStreamsFrom = 4e6f;
 static bool streams_out(const ProductArgs& a, int64_t row_bytes, float compute_us) {
     const int os = a.out_dtype == DGCN_F32 ? 4 : 2;
     const float out = out_bytes(a), all = out + weight_bytes(a, row_bytes) + (float)a.rows * row_bytes;
-    return all / kBytesPerUs > .75f * compute_us && out > .5f * all && a.ldy * os % 64 == 0 && (uintptr_t)a.Y % 64 == 0;
+    return out > kStreamsFrom && all / kBytesPerUs > .75f * compute_us && out > .5f * all && a.ldy * os % 64 == 0 && (uintptr_t)a.Y % 64 == 0;
 }
 
 static int choose_shape(ProductArgs& a, int64_t row_bytes, bool direct) {

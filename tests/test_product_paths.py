@@ -96,6 +96,13 @@ def test_a_call_of_few_tiles_costs_one_at_least(kind):
     assert _path("int8", 100, 4096, 200, 0, "float32") == 16
 
 
+def test_small_outputs_stay_in_the_caches():
+    streams = lambda kind, rows, cin, ctot, groups: _path(kind, rows, cin, ctot, groups, "float32") & 32
+    assert not streams("int8", 154, 16, 64, 0) and streams("int8", 100000, 128, 256, 0)
+    for rows, want in ((154, 0), (1000, 0), (4000, 0), (15000, 0), (20000, 32), (100000, 32)):
+        assert streams("float32", rows, 32, 64, 10) == want, rows
+
+
 @pytest.mark.parametrize("kw,text", [(dict(dtype=9), "unknown dtype"), (dict(dtype=_lib.I8, precise=1), "no such"), (dict(rows=0), "no such"), (dict(out=_lib.F16), "no such"),
                                      (dict(groups=0), "no such"), (dict(dtype=_lib.BF16, out=_lib.BF16, H=None), "no such"), (dict(ldh=3), "bad sizes"),
                                      (dict(cin=0), "bad sizes"), (dict(rows=2 ** 31 - 1), "more than")])
