@@ -87,8 +87,8 @@ class DeviceModel:
 class ModelBank:
     """Several models of one architecture on the device, for batches whose graphs belong to different models
     (``Engine.forward_bank`` / ``solve_bank``; ``Engine.model_bank`` makes one).  ``layers`` = per layer {"weights": float32
-    [models, 2 * out, in] (both supports' weights, an output column's weights contiguous), "bias": None | float32
-    [models, 2 * out] (0 behind the first half), "act", "in", "out", "q" / "scale": the 8-bit form or None}."""
+    [models, 2 * out, in] (both supports' weights, an output column's weights contiguous) or None where the 8-bit form stands for them,
+    "bias": None | float32 [models, 2 * out] (0 behind the first half), "act", "in", "out", "q" / "scale": the 8-bit form or None}."""
 
     def __init__(self, layers, num_models: int, precision: str):
         self.layers, self.num_models, self.precision = layers, num_models, precision
@@ -568,7 +568,7 @@ class Engine:
             q = scale = None
             if precision == "int8" and 0 < l < len(models[0]) - 1:
                 q, scale = self.quantize_rows(W.reshape(-1, fin))
-                q, scale = q.reshape(W.shape), scale.reshape(W.shape[:2])
+                q, scale, W = q.reshape(W.shape), scale.reshape(W.shape[:2]), None
             layers.append({"weights": W, "bias": bias, "act": proto.get("act"), "in": int(fin), "out": int(fout), "q": q, "scale": scale})
         return ModelBank(layers, len(models), precision)
 

@@ -139,6 +139,14 @@ def test_supports_from_elsewhere_have_no_faults(host):
     host.forward_bank(b, host.bank, host.of)
 
 
+def test_an_8_bit_layer_keeps_one_form_of_its_weights(host):
+    models = [datagen.random_model(3, 4, seed=s) for s in (1, 2)]
+    first, hidden, last = host.model_bank(models, precision="int8").layers
+    assert hidden["weights"] is None and tuple(hidden["q"].shape) == (2, 8, 4) and tuple(hidden["scale"].shape) == (2, 8)
+    for layer in (first, last):
+        assert layer["weights"] is not None and layer["q"] is None and layer["scale"] is None
+
+
 @pytest.fixture()
 def checks():
     """An Engine on the host whose argument checks run; a call that passes them all raises AssertionError("accepted")."""
