@@ -45,7 +45,7 @@ class _Lib:
     def dgcn_lgs_batch(self, *a):
         return 0
 
-    dgcn_transform_grouped_batch = None  # (never reached: the Engine's _launch is stood in for)
+    dgcn_transform_grouped_batch = dgcn_quantize_rows_batch = None  # (never reached: the Engine's _launch is stood in for)
 
 
 @pytest.fixture()
