@@ -104,6 +104,8 @@ def _matrix(x, what, dtypes, cols=None, rows=None):
         raise ValueError("%s has shape %s, expected [%s, %s]" % (what, tuple(shape), "rows" if rows is None else rows,
                                                                  "columns" if cols is None else cols))
     r, c = shape
+    if (r | c) >> 31:
+        raise ValueError("%s has shape %s: rows and columns are numbers of 32 bits" % (what, tuple(shape)))
     ld, inner = x.stride()
     if inner != 1 and c > 1:
         raise ValueError("%s: the entries of a row must be contiguous" % what)
@@ -374,6 +376,8 @@ class Engine:
         if not W.is_contiguous():
             raise ValueError("the weights must be contiguous")
         M, ctot, cin = shape if grouped else (1, *shape)
+        if (M | ctot | cin | (rows or 0)) >> 31:
+            raise ValueError("weights of shape %s, %s rows: sizes are numbers of 32 bits" % (tuple(shape), rows))
         ldh = cin
         if H is not None:
             rows, _, ldh = _matrix(H, "H", (W.dtype,), cols=cin, rows=rows)
@@ -394,6 +398,8 @@ class Engine:
         if len(shape) != 1 or shape[0] < 1:
             raise ValueError("group_ptr has shape %s, expected [groups + 1]" % (tuple(shape),))
         G = shape[0] - 1
+        if G >> 31:
+            raise ValueError("%d groups: their number has 32 bits" % G)
         _array(group_ptr, "group_ptr", t.int32, shape)
         if model_of_group is not None:
             _array(model_of_group, "model_of_group", t.int32, (G,))

@@ -221,3 +221,23 @@ def test_empty_outputs_share_nothing(checks):
     _taken(e.transform_grouped, H=z(0, 4), W=z(1, 10, 4), group_ptr=torch.zeros(2, dtype=torch.int32), bias=buf[:10].view(1, 10), out=buf[:0].view(0, 10),
            status=torch.zeros(1, dtype=torch.int32))
     _taken(e.quantize_rows, X=z(0, 4), out=(z(0, 4, dtype=torch.int8), z(0)))
+
+
+def test_sizes_beyond_32_bits_are_refused(checks):
+    """They reach the library as 32-bit numbers: 2^32 + 5 rows would be five."""
+    import torch
+    e, big = checks, 2 ** 32 + 5
+    m = lambda *shape, **kw: torch.empty(*shape, device="meta", **kw)
+    i8 = dict(dtype=torch.int8)
+    word, ptr = torch.zeros(1, dtype=torch.int32), torch.tensor([0, 4], dtype=torch.int32)
+    calls = [lambda: e.quantize_rows(m(big, 1)), lambda: e.quantize_rows(m(1, big)), lambda: e.quantize_rows(m(3, big, dtype=torch.float16)),
+             lambda: e.transform_int8(m(big, 4, **i8), m(big), m(3, 4, **i8), m(3)), lambda: e.transform_int8(m(2, big, **i8), m(2), m(3, big, **i8), m(3)),
+             lambda: e.transform_int8(m(2, 4, **i8), m(2), m(big, 4, **i8), m(big)),
+             lambda: e.transform_grouped(m(big, 4), m(1, 3, 4), ptr, status=word), lambda: e.transform_grouped(m(4, 4), m(big, 3, 4), ptr, status=word),
+             lambda: e.transform_grouped(m(4, 4), m(1, big, 4), ptr, status=word), lambda: e.transform_grouped(None, m(1, 3, 4), ptr, rows=big, status=word),
+             lambda: e.transform_grouped(None, m(1, 3, big), ptr, rows=4, status=word),
+             lambda: e.transform_grouped(m(4, 4), m(1, 3, 4), m(big + 1, dtype=torch.int32), model_of_group=m(big, dtype=torch.int32), status=word),
+             lambda: e.transform_grouped_int8(m(big, 4, **i8), m(big), m(1, 3, 4, **i8), m(1, 3), ptr, status=word)]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
