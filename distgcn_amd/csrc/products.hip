@@ -371,7 +371,7 @@ constexpr int kRowBytes = 128;  // bytes of k per stage and row
 // Large products are bound by the matrix pipe and the LDS reads that feed it: int8 8 192 x 4 096 x 4 096 in 119 us (2.3 POP/s, as a large
 // library product; pipe busy in 57 % of the cycles, 256 x 256 tiles), bf16 8 192 rows in 8 groups, 2 048 x 4 096 in 149 us (192 x 256).
 // Narrow ones are a copy: 100 000 rows int8 128 -> 256 float32 in 24 us (115 MB, 64 x 64).
-// A stage is worked off in phases (64 bytes of k x up to four row tiles).  AHEAD (the largest tile, two waves per SIMD): a phase's
+// A stage is worked off in phases (64 bytes of k x up to four row tiles).  AHEAD (every tile of eight waves, two per SIMD): a phase's
 // fragments are requested behind the first MFMAs of the phase in front of it, across the stage's barrier too, so the matrix pipe
 // does not wait for LDS; smaller tiles have more waves to hide that.  Row tiles behind the group's last row are skipped four at a time.
 template <int KIND, int BM, int BN, int WM, int WN, int NBUF, bool DIRECT>
@@ -872,10 +872,12 @@ enum Path {
     P_ROWS_16, P_ROWS_32,                                 // k_product_rows, up to 16 / 32 columns
 };
 
-// The tile shapes of the 8- and 16-bit products and what they cost, fitted to 26 shapes of 128 .. 100 000 rows, k of 64 .. 4 096 bytes and
+// The tile shapes of the 8- and 16-bit products and what they cost, fitted to shapes of 128 .. 100 000 rows, k of 64 .. 4 096 bytes and
 // 20 .. 4 096 columns, dense and in 8 .. 300 groups: a stage (128 bytes of k) takes s1 us in a workgroup that has its CU to itself and sc
-// us with per_cu of them there, a tile's start and end f us.  The least estimate is the fastest shape or within 14 % of it on 22 of the
-// 26 (the others: many groups of few rows, up to 35 %).
+// us with per_cu of them there, a tile's start and end f us.  The choice is the fastest shape or within 11 % of it on 32 of 36 calls
+// (profiles/products_shapes.txt: every shape's time beside its estimate).  The others lose up to 40 %: the host knows how many tiles to
+// expect, not how many there are, and two more than a full round of workgroups are another round (16 000 rows of 2 048 bytes in 8 groups,
+// 512 columns: 39.5 us with 128 x 256, 28.2 with 192 x 256).
 struct Shape { int bm, bn, per_cu; float s1, sc, f; };
 constexpr int kShapes = 5;
 constexpr float kBytesPerUs = 4.7e6f;  // a large copy, read and written
@@ -917,7 +919,7 @@ static int choose_shape(ProductArgs& a, int64_t row_bytes, bool direct) {
         if (!p.bm) continue;
         const float per = expected_slots(a, p.bm) * (float)((a.ctot + p.bn - 1) / p.bn) / kCUs;  // tiles per CU
         const float rounds = floorf(per / p.per_cu), rest = per - rounds * p.per_cu;
-        float cost = rounds * (p.sc * steps + p.f);
+        float cost = rounds * (p.sc * steps + p.f);  // (the expected count is a mean: up to .02 tiles per CU behind a round are left out)
         if (rest > .02f || rounds == 0.f) cost += (p.s1 + (p.per_cu > 1 ? (p.sc - p.s1) * (ceilf(rest) - 1.f) / (p.per_cu - 1) : 0.f)) * steps + p.f;
         if (cost < least) { least = cost; best = i; }
     }
