@@ -1,6 +1,6 @@
 #!/bin/bash
 # The -DDGCN_DIAG profiling build of the library (phase clocks / ablation switches in k_fused; tools/stamp_fused.py).
-# Not part of the product: built on demand (here or on the GPU box: hipcc cross-compiles), selected with
+# Not part of the product: built on demand (hipcc cross-compiles), selected with
 # DGCN_LIB=distgcn_amd/libdgcn_diag.so.  One object per source, side by side, like __graft_entry__.build().
 set -e
 . "$(dirname "$0")/library_build.sh"
