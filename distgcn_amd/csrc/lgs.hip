@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256) void k_margin_risk(const int32_t* __restrict__
             const double pv = pri(v), wv = wabs(v);
             for (int j = row_ptr[v] + sub; j < row_ptr[v + 1]; j += 8) {
                 const int u = col_idx[j];
-                if (state[u] == 1) safe |= (pri(u) - pv) > delta * (wabs(u) + wv);
+                if ((unsigned)(u - n0) < (unsigned)(n1 - n0) && state[u] == 1) safe |= (pri(u) - pv) > delta * (wabs(u) + wv);
             }
         }
         safe |= __shfl_xor((int)safe, 1) != 0;

@@ -92,6 +92,26 @@ def test_greedy_search_stays_inside_its_graph(engine, sizes, degree, kw):
             assert torch.equal(state, a["state"][lo:hi]) and int(a["rounds"][g]) == int(b["rounds"][g])
 
 
+def test_margin_risk_stays_inside_its_graph(engine):
+    """A column outside the graph is nobody's member neighbour."""
+    import torch
+    good, bad = _batch_with_columns([30, 50, 20, 70], 1, FAR)
+    prio = torch.from_numpy(np.random.default_rng(5).random(good.num_nodes)).cuda()
+    a, b = engine.upload(good), engine.upload(bad)
+    state = engine.lgs(a, prio=prio)["state"]
+    want, got = (engine.margin_risk(x, state, 1e-3, prio=prio).cpu().numpy() for x in (a, b))
+    assert want[0] == got[0] and want[2] == got[2]
+    # by the definition: an excluded vertex is safe iff a member neighbour is ahead by more than twice delta
+    st, p = state.cpu().numpy(), prio.cpu().numpy()
+    for g, (lo, hi) in enumerate(bad.graph_slices()):
+        risky = 0
+        for v in range(lo, hi):
+            near = bad.col_idx[bad.row_ptr[v]:bad.row_ptr[v + 1]]
+            near = near[(near >= lo) & (near < hi)]
+            risky += st[v] == 2 and not any(st[u] == 1 and p[u] - p[v] > 2e-3 for u in near)
+        assert got[g] == risky, g
+
+
 def _self_loop_batch():
     from distgcn_amd.batch import HostBatch
     adjs, wts = _graphs([30, 50, 20], 2)
